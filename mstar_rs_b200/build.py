@@ -1,6 +1,6 @@
 """Build the sampler's CUDA library in-tree for sm_100a.
 
-`python -m mstar_rs_b200.build` compiles csrc/sampler.cu with nvcc into
+`python -m mstar_rs_b200.build` compiles csrc/*.cu with nvcc into
 mstar_rs_b200/_lib/libmstar_sampler.so (C ABI declared in
 include/mstar_sampler.h).  The library links the CUDA runtime statically, so
 it needs only the driver at load time.
@@ -14,8 +14,9 @@ import sys
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
-SRC = [os.path.join(PKG, "csrc", "sampler.cu")]
-DEPS = SRC + [os.path.join(PKG, "csrc", "spec.cuh"), os.path.join(PKG, "csrc", "lmhead.cuh"), os.path.join(ROOT, "include", "mstar_sampler.h")]
+CSRC = os.path.join(PKG, "csrc")
+SRC = [os.path.join(CSRC, n) for n in ("sampler.cu",)]
+DEPS = [os.path.join(CSRC, n) for n in sorted(os.listdir(CSRC))] + [os.path.join(ROOT, "include", "mstar_sampler.h")]
 OUT = os.path.join(PKG, "_lib", "libmstar_sampler.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -38,7 +39,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not stale():
         return OUT
     os.makedirs(os.path.dirname(OUT), exist_ok=True)
-    cmd = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
+    cmd = [nvcc(), *ARCH, "--threads", "4", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
            "-I", os.path.join(ROOT, "include"), "-o", OUT + ".tmp", *SRC]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")

@@ -61,7 +61,9 @@
 #include <string>
 
 #include "../../include/mstar_sampler.h"
+#include "common.cuh"
 #include "spec.cuh"
+#include "tcgen05.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -99,11 +101,6 @@ static_assert(TAIL_CAP * 44 + NBK * 12 <= LEAN_SCRATCH, "fast tail scratch");
 static_assert(NBK % NT == 0, "tail bucket scan");
 static_assert(NBK >= 2 * 256 && NBK >= NT, "value-bucket tail: counts and starts over the bucket counts, weights over the masses");
 static_assert(NT == 512, "the rank sort splits 512 threads into 64 / 128 / 256 slots");
-// Bound on one wait for a bulk copy: 2 ms of %globaltimer (a copy of at
-// most 64 KB lands within microseconds), with an iteration cap behind it.
-constexpr uint64_t kWaitNs = 2000000ull;
-constexpr unsigned kWaitIters = 1u << 26;
-
 struct __align__(8) Cand {
   float x;
   uint32_t gid;
@@ -226,10 +223,6 @@ struct CtaSh {
 __device__ __forceinline__ uint64_t u64min(uint64_t a, uint64_t b) { return a < b ? a : b; }
 __device__ __forceinline__ uint64_t u64max(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-
 // First of `cnt` consecutive slots in a shared list for each lane of a full
 // warp (all 32 lanes call it together): one atomic per warp.
 __device__ __forceinline__ uint32_t warp_reserve(uint32_t *counter, uint32_t cnt) {
@@ -267,50 +260,6 @@ __device__ __forceinline__ void cluster_arrive_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
-               "r"(bytes)
-               : "memory");
-}
-
-__device__ __forceinline__ uint64_t global_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-// Bounded wait on phase `parity` (kWaitNs); false if the limit ran out.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
-  const uint32_t a = smem_u32(bar);
-  uint64_t t0 = 0;
-  for (unsigned i = 0; i < kWaitIters; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(a), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    const uint64_t t = global_ns();
-    if (i == 0) t0 = t;
-    else if (t - t0 > kWaitNs) return false;
-  }
-  return false;
-}
-
-__device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
 
 template <typename T>
 struct Elem;
@@ -3694,7 +3643,7 @@ __global__ void __launch_bounds__(NT, 1)
 
 static thread_local std::string g_last_error;
 
-static int fail(int code, const std::string &msg) {
+int fail(int code, const std::string &msg) {
   g_last_error = msg;
   return code;
 }
@@ -3743,10 +3692,9 @@ static int validate(const mstar_sampler_params_t *p) {
 // Device properties the planner reads, cached per device (the calling
 // thread's current device; a process may drive several GPUs, possibly of
 // different kinds) under one lock.
-constexpr int kMaxDevices = 64;
 static std::mutex g_dev_mu;
 
-static int current_device() {
+int current_device() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) dev = 0;
   return dev;
@@ -3766,12 +3714,12 @@ static int device_attr(cudaDeviceAttr what, int (&cache)[kMaxDevices], int fallb
   return cache[dev];
 }
 
-static int max_smem_optin() {
+int max_smem_optin() {
   static int cache[kMaxDevices] = {};
   return device_attr(cudaDevAttrMaxSharedMemoryPerBlockOptin, cache, 232448);
 }
 
-static int sm_count() {
+int sm_count() {
   static int cache[kMaxDevices] = {};
   return device_attr(cudaDevAttrMultiProcessorCount, cache, 148);
 }
