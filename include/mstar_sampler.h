@@ -54,6 +54,7 @@ extern "C" {
 #define MSTAR_STATUS_TIMEOUT 0x10u     /* a bounded wait (2 ms) on a bulk copy gave up; the id is not valid */
 #define MSTAR_STATUS_STOP 0x20u        /* the sampled id is one of the slot's stop ids */
 #define MSTAR_STATUS_BAD_RECORD 0x40u  /* TP merge: a record entry held an id >= V_global (left out) */
+#define MSTAR_STATUS_BAD_ID 0x80u      /* a token id >= V was given (its row counts as a padding row) */
 
 /* return codes */
 #define MSTAR_OK 0
@@ -250,6 +251,104 @@ int mstar_lmhead_logits_static(const void *hidden, const void *weight, int32_t B
 int mstar_sampler_lmhead_step(const mstar_sampler_params_t *p, const void *hidden, const void *weight,
                               int32_t d, void *workspace, int64_t workspace_bytes, uint32_t *status,
                               void *stream);
+
+/* A 4-bit matrix [V, d] with group scales, in plain rows:
+ *   w[v, k] = (q[v, k] - z[v, k / group]) * s[v, k / group]
+ * codes: [V, d / 2] bytes, the even k in the low four bits (16-byte
+ * aligned); scales: [V, d / group] of scale_dtype; zeros: [V, d / group]
+ * bytes in [0, 15] (only the low four bits count), or NULL for 8.  group is
+ * 32, 64 or 128 and divides d. */
+typedef struct mstar_w4 {
+  const void *codes;
+  const void *scales;
+  const void *zeros;
+  int32_t V, d, group, scale_dtype;
+} mstar_w4_t;
+
+/* mstar_lmhead_logits with 4-bit weights: logits[b * ld + v] = sum_k
+ * hidden[b * ld_hidden + k] * w[v, k], hidden bf16, fp32 accumulation (code
+ * minus zero point times hidden is exact; each group's sum is scaled in
+ * fp32), stored as dtype.  B <= 256.  workspace: device scratch of at least
+ * mstar_lmhead_w4_workspace_bytes(B, V, d) bytes, 256-byte aligned; its
+ * contents need not be preserved or initialised, and calls that overlap on
+ * the GPU need their own.  status: NULL or a device word that gets bit 1 if
+ * a bounded in-kernel wait ran out. */
+int64_t mstar_lmhead_w4_workspace_bytes(int32_t B, int32_t V, int32_t d);
+int mstar_lmhead_logits_w4(const void *hidden, int64_t ld_hidden, int32_t B, const mstar_w4_t *w, void *logits,
+                           int32_t dtype, int64_t ld, void *workspace, int64_t workspace_bytes, uint32_t *status,
+                           void *stream);
+
+/* mstar_sampler_lmhead_step with 4-bit weights: mstar_lmhead_logits_w4 into
+ * p->logits, then mstar_sampler_step on it. */
+int mstar_sampler_lmhead_step_w4(const mstar_sampler_params_t *p, const void *hidden, int64_t ld_hidden,
+                                 const mstar_w4_t *w, void *workspace, int64_t workspace_bytes, uint32_t *status,
+                                 void *stream);
+
+/* Embedding lookup, the step's other end (the sampled ids' rows are the
+ * next step's input): out[n, :] = scale * table[ids[n], :], out [N, d] of
+ * out_dtype, table [V, ld] of dtype, or a 4-bit matrix (out 16-byte
+ * aligned).  A negative id is a padding row and gives zeros; an id >= V
+ * does too and sets MSTAR_STATUS_BAD_ID in *status (NULL or a device word). */
+int mstar_embed_tokens(const int64_t *ids, int64_t N, const void *table, int32_t dtype, int32_t V, int32_t d,
+                       int64_t ld, float scale, void *out, int32_t out_dtype, uint32_t *status, void *stream);
+int mstar_embed_tokens_w4(const int64_t *ids, int64_t N, const mstar_w4_t *w, float scale, void *out,
+                          int32_t out_dtype, uint32_t *status, void *stream);
+
+/* The lookup's gradient to the table: out[v, :] = base[v, :] + scale * sum
+ * over n with ids[n] == v of dout[n, :], every row of out [V, d] written
+ * (base NULL: rows without a token are zeros).  base has out's type and may
+ * be out itself (the sums are added in place), otherwise it must not overlap
+ * it.  fp32 sums in a fixed order, rounded once.  dout [N, ld] of dtype.
+ * workspace: mstar_embed_grad_workspace_bytes(N, V, d) bytes, 256-byte
+ * aligned, as for mstar_lmhead_logits_w4.  Ids as for the lookup. */
+int64_t mstar_embed_grad_workspace_bytes(int32_t N, int32_t V, int32_t d);
+int mstar_embed_tokens_grad(const int64_t *ids, int32_t N, const void *dout, int32_t dtype, int64_t ld, int32_t V,
+                            int32_t d, float scale, const void *base, void *out, int32_t out_dtype, void *workspace,
+                            int64_t workspace_bytes, uint32_t *status, void *stream);
+
+/* Log-probabilities of given ids under softmax(logits / temperature):
+ * lse[n] = log sum_v exp(logits[n, v] / temperature) (or NULL) and logp[n] =
+ * logits[n, ids[n]] / temperature - lse[n].  -inf logits are masked ids; a
+ * row of nothing else is empty: lse and logp are -inf and *status gets
+ * MSTAR_STATUS_EMPTY.  NaN and +inf make their row NaN.  A negative id is a
+ * padding row with logp 0; an id >= V counts as one and sets
+ * MSTAR_STATUS_BAD_ID.  temperature in [1e-5, 1e5]. */
+int mstar_token_logprobs(const void *logits, int32_t dtype, int32_t N, int32_t V, int64_t ld, const int64_t *ids,
+                         double temperature, float *logp, float *lse, uint32_t *status, void *stream);
+
+/* The gradient of sum_n dlogp[n] * logp[n] to the logits: dlogits[n, v] =
+ * dlogp[n] / temperature * ([v == ids[n]] - exp(logits[n, v] / temperature -
+ * lse[n])), of the logits' type; dlogits may be logits itself (replaced in
+ * place), otherwise it must not overlap it.  Padding and empty rows: zeros. */
+int mstar_token_logprobs_grad(const void *logits, int32_t dtype, int32_t N, int32_t V, int64_t ld, const int64_t *ids,
+                              double temperature, const float *lse, const float *dlogp, void *dlogits,
+                              int64_t ld_dlogits, void *stream);
+
+/* Clipped policy loss of sampled tokens and its gradient, in one pass:
+ *   r = exp(logp - old_logp)                       (old_logp NULL: r = 1)
+ *   loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *          + kl_coef (exp(ref_logp - logp) - (ref_logp - logp) - 1)
+ *   dlogits = d(sum_n weights[n] loss[n]) / dlogits   (weights NULL: 1)
+ * logp as in mstar_token_logprobs.  Padding and empty rows have loss 0 and a
+ * zero gradient, and so has the gradient of an id whose logit is masked. */
+typedef struct mstar_policy_params {
+  const void *logits;        /* [N, ld] of dtype */
+  int32_t dtype, N, V, pad0;
+  int64_t ld;
+  const int64_t *ids;        /* [N] */
+  const float *old_logp;     /* [N] or NULL */
+  const float *ref_logp;     /* [N], or NULL with kl_coef 0 */
+  const float *advantages;   /* [N] */
+  const float *weights;      /* [N] or NULL */
+  double temperature;        /* in [1e-5, 1e5] */
+  double clip_low, clip_high, kl_coef;
+  float *loss, *logp;        /* [N] each */
+  float *lse;                /* [N] or NULL (padding rows: 0) */
+  void *dlogits;             /* [N, ld_dlogits] of dtype, logits itself, or NULL: no gradient */
+  int64_t ld_dlogits;
+  uint32_t *status;          /* NULL or a device word */
+} mstar_policy_params_t;
+int mstar_policy_loss(const mstar_policy_params_t *p, void *stream);
 
 /* The sampler's Philox4x32-10 uniform for (seed, offset), computed on the
  * host; lets callers reproduce a draw without a device. */

@@ -26,10 +26,12 @@ STATUS_TP_OVERFLOW = 0x8
 STATUS_TIMEOUT = 0x10
 STATUS_STOP = 0x20
 STATUS_BAD_RECORD = 0x40
+STATUS_BAD_ID = 0x80
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA = 0, 1, 2, 3
 
 P = ctypes.c_void_p
 I32, I64, U32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32
+F32, F64 = ctypes.c_float, ctypes.c_double
 
 
 class Params(ctypes.Structure):
@@ -52,6 +54,24 @@ class Params(ctypes.Structure):
     ]
 
 
+class W4(ctypes.Structure):
+    """Mirror of `mstar_w4_t`."""
+
+    _fields_ = [("codes", P), ("scales", P), ("zeros", P),
+                ("V", I32), ("d", I32), ("group", I32), ("scale_dtype", I32)]
+
+
+class PolicyParams(ctypes.Structure):
+    """Mirror of `mstar_policy_params_t`."""
+
+    _fields_ = [
+        ("logits", P), ("dtype", I32), ("N", I32), ("V", I32), ("pad0", I32), ("ld", I64), ("ids", P),
+        ("old_logp", P), ("ref_logp", P), ("advantages", P), ("weights", P),
+        ("temperature", F64), ("clip_low", F64), ("clip_high", F64), ("kl_coef", F64),
+        ("loss", P), ("logp", P), ("lse", P), ("dlogits", P), ("ld_dlogits", I64), ("status", P),
+    ]
+
+
 class SamplerError(RuntimeError):
     pass
 
@@ -66,6 +86,9 @@ EXPORTS = (
     "mstar_lmhead_workspace_bytes", "mstar_lmhead_logits", "mstar_sampler_lmhead_step",
     "mstar_lmhead_logits_static", "mstar_sampler_tp_local2", "mstar_sampler_tp_merge1", "mstar_sampler_tp_mass",
     "mstar_sampler_tp_merge2",
+    "mstar_lmhead_w4_workspace_bytes", "mstar_lmhead_logits_w4", "mstar_sampler_lmhead_step_w4",
+    "mstar_embed_tokens", "mstar_embed_tokens_w4", "mstar_embed_grad_workspace_bytes", "mstar_embed_tokens_grad",
+    "mstar_token_logprobs", "mstar_token_logprobs_grad", "mstar_policy_loss",
 )
 
 
@@ -112,6 +135,19 @@ def lib() -> ctypes.CDLL:
         L.mstar_sampler_lmhead_step.restype = ctypes.c_int
         L.mstar_lmhead_logits_static.argtypes = [P, P, I32, I32, I32, P, I32, I64, P, P]
         L.mstar_lmhead_logits_static.restype = ctypes.c_int
+        W4P = ctypes.POINTER(W4)
+        L.mstar_lmhead_w4_workspace_bytes.argtypes = [I32, I32, I32]
+        L.mstar_lmhead_w4_workspace_bytes.restype = I64
+        L.mstar_lmhead_logits_w4.argtypes = [P, I64, I32, W4P, P, I32, I64, P, I64, P, P]
+        L.mstar_sampler_lmhead_step_w4.argtypes = [ctypes.POINTER(Params), P, I64, W4P, P, I64, P, P]
+        L.mstar_embed_tokens.argtypes = [P, I64, P, I32, I32, I32, I64, F32, P, I32, P, P]
+        L.mstar_embed_tokens_w4.argtypes = [P, I64, W4P, F32, P, I32, P, P]
+        L.mstar_embed_grad_workspace_bytes.argtypes = [I32, I32, I32]
+        L.mstar_embed_grad_workspace_bytes.restype = I64
+        L.mstar_embed_tokens_grad.argtypes = [P, I32, P, I32, I64, I32, I32, F32, P, P, I32, P, I64, P, P]
+        L.mstar_token_logprobs.argtypes = [P, I32, I32, I32, I64, P, F64, P, P, P, P]
+        L.mstar_token_logprobs_grad.argtypes = [P, I32, I32, I32, I64, P, F64, P, P, P, I64, P]
+        L.mstar_policy_loss.argtypes = [ctypes.POINTER(PolicyParams), P]
         L.mstar_sampler_philox_uniform.argtypes = [ctypes.c_uint64, ctypes.c_uint64]
         L.mstar_sampler_philox_uniform.restype = ctypes.c_float
         if L.mstar_sampler_abi_version() != ABI_VERSION:

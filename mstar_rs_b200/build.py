@@ -15,7 +15,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
-SRC = [os.path.join(CSRC, n) for n in ("sampler.cu",)]
+SRC = [os.path.join(CSRC, n) for n in ("sampler.cu", "w4head.cu", "token_rows.cu", "embedding.cu")]
 DEPS = [os.path.join(CSRC, n) for n in sorted(os.listdir(CSRC))] + [os.path.join(ROOT, "include", "mstar_sampler.h")]
 OUT = os.path.join(PKG, "_lib", "libmstar_sampler.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -8,6 +8,8 @@
 #include <cstdint>
 #include <string>
 
+#include "../../include/mstar_sampler.h"
+
 namespace mstar {
 
 // Bound on one wait for a bulk copy: 2 ms of %globaltimer (a copy of at
@@ -71,5 +73,6 @@ int fail(int code, const std::string &msg);  // keeps `msg` for mstar_sampler_la
 int current_device();
 int sm_count();
 int max_smem_optin();
+int check_w4(const mstar_w4_t *w);  // a 4-bit matrix's sizes and pointers (w4head.cu)
 
 }  // namespace mstar

@@ -1,0 +1,603 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens: the other
+// end of the LM head's table.
+//
+//   out[n] = scale * table[ids[n]]          (a negative id: a row of zeros)
+//   grad[v] = base[v] + scale * sum over n with ids[n] = v of dout[n]
+//
+// Lookup: a copy bound by memory; every thread moves one vector of eight
+// values (from 16 or 32 bytes of a plain table, 4 of a 4-bit one) for several
+// (row, column) places at once.
+//
+// Gradient: the tokens are sorted by id first, so each row of the table is
+// summed by one owner in position order (no atomics on values: the same
+// inputs give the same bits) and every row of the output is written once.
+//   sort   each CTA takes a range of ids and reads all ids twice: once to
+//          count (per id and per warp, each warp owning a contiguous part of
+//          the positions), once to place.  It counts the ids below its range
+//          as it goes, so CTAs need nothing of one another.
+//   sums   the sorted positions in chunks of equal length, whatever the ids'
+//          frequencies; runs inside a chunk are written, runs that cross a
+//          border leave 32-bit partial sums.  Further CTAs of the same launch
+//          write the rows that no token has.
+//   joins  the chunk in which a crossing run starts adds its parts in order.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace mstar {
+namespace emb {
+
+constexpr int NT = 256;
+
+// W consecutive values as one access (W = 8: 16 bytes of bf16, two of 16 of f32).
+template <int W>
+__device__ __forceinline__ void load(const float *p, float (&x)[W]) {
+  if constexpr (W == 8) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else if constexpr (W == 2) {
+    const float2 a = __ldg(reinterpret_cast<const float2 *>(p));
+    x[0] = a.x, x[1] = a.y;
+  } else {
+    x[0] = __ldg(p);
+  }
+}
+template <int W>
+__device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&x)[W]) {
+  if constexpr (W == 8) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+  } else if constexpr (W == 2) {
+    const uint32_t u = __ldg(reinterpret_cast<const uint32_t *>(p));
+    x[0] = __uint_as_float(u << 16);
+    x[1] = __uint_as_float(u & 0xFFFF0000u);
+  } else {
+    x[0] = __bfloat162float(p[0]);
+  }
+}
+template <int W>
+__device__ __forceinline__ void store(float *p, const float (&x)[W]) {
+  if constexpr (W == 8) {
+    __stcs(reinterpret_cast<float4 *>(p), make_float4(x[0], x[1], x[2], x[3]));
+    __stcs(reinterpret_cast<float4 *>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
+  } else if constexpr (W == 2) {
+    *reinterpret_cast<float2 *>(p) = make_float2(x[0], x[1]);
+  } else {
+    *p = x[0];
+  }
+}
+template <int W>
+__device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&x)[W]) {
+  if constexpr (W == 8) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    __stcs(reinterpret_cast<uint4 *>(p), make_uint4(u[0], u[1], u[2], u[3]));
+  } else if constexpr (W == 2) {
+    *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(x[0], x[1]);
+  } else {
+    *p = __float2bfloat16_rn(x[0]);
+  }
+}
+
+// ------------------------------------------------------------ lookup
+
+struct Lookup {
+  const void *table;
+  int64_t ld;  // table row stride in values
+  const int64_t *ids;
+  int64_t N;
+  int32_t V, d;
+  float scale;
+  void *out;  // [N, d]
+  uint32_t *status;
+  // 4-bit tables
+  const uint8_t *codes;
+  const void *scales;
+  const uint8_t *zeros;
+  int32_t scale_dtype, group_log2, ngroups;
+};
+
+__device__ __forceinline__ void bad_id(const Lookup &a, int64_t id, int col) {
+  if (id >= a.V && col == 0 && a.status) atomicOr(a.status, MSTAR_STATUS_BAD_ID);
+}
+
+template <typename TI, typename TO, int W>
+__global__ void __launch_bounds__(NT) embed_kernel(const Lookup a) {
+  constexpr int U = 4;
+  const uint32_t per = (uint32_t)(a.d / W);
+  const int64_t total = a.N * (int64_t)per;
+  const int64_t i0 = (int64_t)blockIdx.x * (NT * U) + threadIdx.x;
+  float x[U][W];
+  int64_t at[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = i0 + u * NT;
+    at[u] = -1;
+    if (i >= total) continue;
+    const int64_t n = i / per;
+    const int col = (int)(i - n * per) * W;
+    const int64_t id = a.ids[n];
+    at[u] = n * a.d + col;
+    bad_id(a, id, col);
+    if (id >= 0 && id < a.V) {
+      load<W>(static_cast<const TI *>(a.table) + id * a.ld + col, x[u]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j) x[u][j] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (at[u] < 0) continue;
+#pragma unroll
+    for (int j = 0; j < W; ++j) x[u][j] *= a.scale;
+    store<W>(static_cast<TO *>(a.out) + at[u], x[u]);
+  }
+}
+
+// Eight values (one word of codes, all of one group) per place.
+template <typename TO>
+__global__ void __launch_bounds__(NT) embed_w4_kernel(const Lookup a) {
+  constexpr int U = 4;
+  const uint32_t per = (uint32_t)a.d / 8;
+  const int64_t total = a.N * (int64_t)per;
+  const int64_t i0 = (int64_t)blockIdx.x * (NT * U) + threadIdx.x;
+  uint32_t w[U];
+  float s[U], z[U];
+  int64_t at[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = i0 + u * NT;
+    at[u] = -1;
+    if (i >= total) continue;
+    const int64_t n = i / per;
+    const int col = (int)(i - n * per) * 8;
+    const int64_t id = a.ids[n];
+    at[u] = n * a.d + col;
+    w[u] = 0u;
+    s[u] = z[u] = 0.f;
+    bad_id(a, id, col);
+    if (id < 0 || id >= a.V) continue;
+    w[u] = __ldg(reinterpret_cast<const uint32_t *>(a.codes + id * (a.d / 2) + col / 2));
+    const int64_t g = id * a.ngroups + (col >> a.group_log2);
+    s[u] = a.scale_dtype == MSTAR_DTYPE_F32 ? __ldg(static_cast<const float *>(a.scales) + g)
+                                            : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.scales)[g]);
+    z[u] = a.zeros ? (float)(__ldg(a.zeros + g) & 15) : 8.f;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (at[u] < 0) continue;
+    float x[8];
+    // (q - z) s as stored weights are used elsewhere, then the lookup's scale
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = ((float)((w[u] >> (4 * j)) & 15u) - z[u]) * s[u] * a.scale;
+    store<8>(static_cast<TO *>(a.out) + at[u], x);
+  }
+}
+
+// ------------------------------------------------------------ gradient
+
+constexpr int SORT_NT = 1024;
+constexpr int SORT_NW = SORT_NT / 32;
+constexpr int MAX_BINS = 1088;  // ids per CTA of the sort: 156940 ids fit 148 CTAs
+constexpr int SUM_NT = 128;
+
+struct Grad {
+  const void *dout;
+  int64_t ldo;  // dout row stride in values
+  const int64_t *ids;
+  int32_t N, V, d;
+  float scale;
+  const void *base;  // [V, d] of the output's type, or NULL
+  void *out;         // [V, d]
+  uint32_t *status;
+  int32_t bins;      // ids per CTA of the sort
+  int32_t chunk, nchunks, col_tiles, zero_rows, nzero;
+  int32_t *start;    // [V + 1] first sorted place of each id
+  int32_t *pos;      // [N] positions, sorted by id, then by position
+  int32_t *key;      // [N] their ids
+  float *part;       // [nchunks][2][d]: a run from the chunk before / into the chunk after
+};
+
+__global__ void __launch_bounds__(SORT_NT) sort_tokens_kernel(const Grad a) {
+  extern __shared__ int32_t cnt[];  // [SORT_NW][bins]
+  __shared__ int32_t below_w[SORT_NW], scan_w[SORT_NW];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int base = (int)blockIdx.x * a.bins, bins = min(a.bins, a.V - base);
+  for (int i = tid; i < SORT_NW * a.bins; i += SORT_NT) cnt[i] = 0;
+  __syncthreads();
+  const int n0 = (int)((int64_t)a.N * warp / SORT_NW), n1 = (int)((int64_t)a.N * (warp + 1) / SORT_NW);
+  int32_t *mine = cnt + warp * a.bins;
+  int below = 0;
+  bool bad = false;
+  constexpr int U = 8;
+  for (int n = n0 + lane; n < n1; n += 32 * U) {
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = n + 32 * u < n1 ? __ldg(a.ids + n + 32 * u) : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      below += id[u] >= 0 && id[u] < base;
+      bad |= id[u] >= a.V;
+      if (id[u] >= base && id[u] < base + bins) atomicAdd(&mine[(int)id[u] - base], 1);
+    }
+  }
+  if (bad && blockIdx.x == 0 && a.status) atomicOr(a.status, MSTAR_STATUS_BAD_ID);
+  for (int o = 16; o; o >>= 1) below += __shfl_xor_sync(~0u, below, o);
+  if (lane == 0) below_w[warp] = below;
+  __syncthreads();
+  int first = 0;
+  for (int w = 0; w < SORT_NW; ++w) first += below_w[w];
+  // exclusive prefix over the ids, then over the warps of each id
+  for (int b0 = 0; b0 < bins; b0 += SORT_NT) {
+    const int b = b0 + tid;
+    int tot = 0;
+    if (b < bins)
+      for (int w = 0; w < SORT_NW; ++w) tot += cnt[w * a.bins + b];
+    int inc = tot;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(~0u, inc, o);
+      if (lane >= o) inc += t;
+    }
+    if (lane == 31) scan_w[warp] = inc;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < SORT_NW; ++w) {
+      if (w < warp) before += scan_w[w];
+      all += scan_w[w];
+    }
+    int at = first + before + inc - tot;
+    if (b < bins) {
+      a.start[base + b] = at;
+      for (int w = 0; w < SORT_NW; ++w) {
+        const int t = cnt[w * a.bins + b];
+        cnt[w * a.bins + b] = at;
+        at += t;
+      }
+    }
+    first += all;
+    __syncthreads();
+  }
+  if (tid == 0 && base + bins == a.V) a.start[a.V] = first;
+  for (int nb = n0; nb < n1; nb += 32 * U) {
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = nb + 32 * u + lane < n1 ? __ldg(a.ids + nb + 32 * u + lane) : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = id[u] >= base && id[u] < base + bins;
+      const unsigned any = __ballot_sync(~0u, in);
+      if (!any) continue;
+      const int b = in ? (int)id[u] - base : -1;
+      const unsigned same = __match_any_sync(~0u, b);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      int at = 0;
+      if (in) at = mine[b] + rank;
+      __syncwarp();
+      if (in && rank == 0) mine[b] = at + __popc(same);
+      __syncwarp();
+      if (in) {
+        a.pos[at] = nb + 32 * u + lane;
+        a.key[at] = (int)id[u];
+      }
+    }
+  }
+}
+
+template <typename TO, int W>
+__device__ __forceinline__ void finish(const Grad &a, int v, int col, float (&acc)[W]) {
+  const int64_t at = (int64_t)v * a.d + col;
+#pragma unroll
+  for (int j = 0; j < W; ++j) acc[j] *= a.scale;
+  if (a.base) {
+    float b[W];
+    load<W>(static_cast<const TO *>(a.base) + at, b);
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[j] += b[j];
+  }
+  store<W>(static_cast<TO *>(a.out) + at, acc);
+}
+
+template <typename TI, typename TO, int W>
+__global__ void __launch_bounds__(SUM_NT) sum_tokens_kernel(const Grad a) {
+  const int work = a.nchunks * a.col_tiles;
+  if ((int)blockIdx.x >= work) {  // rows without a token: zeros, or the base's own
+    const int r0 = ((int)blockIdx.x - work) * a.zero_rows;
+    for (int v = r0; v < min(a.V, r0 + a.zero_rows); ++v) {
+      if (a.start[v + 1] > a.start[v]) continue;
+      for (int col = (int)threadIdx.x * W; col < a.d; col += SUM_NT * W) {
+        float acc[W] = {};
+        finish<TO, W>(a, v, col, acc);
+      }
+    }
+    return;
+  }
+  const int c = (int)blockIdx.x / a.col_tiles;
+  const int col = (((int)blockIdx.x % a.col_tiles) * SUM_NT + (int)threadIdx.x) * W;
+  const int total = a.start[a.V];
+  const int s0 = c * a.chunk, s1 = min(total, s0 + a.chunk);
+  if (col >= a.d || s0 >= s1) return;
+  constexpr int U = 4;
+  float acc[W] = {};
+  bool from_before = s0 > 0 && a.key[s0 - 1] == a.key[s0];
+  for (int s = s0; s < s1; s += U) {
+    float x[U][W];
+    int key[U + 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      key[u] = s + u < s1 ? a.key[s + u] : -1;
+      if (s + u < s1) load<W>(static_cast<const TI *>(a.dout) + (int64_t)a.pos[s + u] * a.ldo + col, x[u]);
+    }
+    key[U] = s + U < total ? a.key[s + U] : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s + u >= s1) break;
+#pragma unroll
+      for (int j = 0; j < W; ++j) acc[j] += x[u][j];
+      const int next = s + u + 1 < total ? (s + u + 1 < s1 || u + 1 == U ? key[u + 1] : a.key[s + u + 1]) : -1;
+      const bool last = s + u + 1 == s1;
+      if (next == key[u] && !last) continue;
+      if (from_before || next == key[u]) {  // the run crosses a border of the chunk
+        float *p = a.part + ((int64_t)c * 2 + (from_before ? 0 : 1)) * a.d + col;
+#pragma unroll
+        for (int j = 0; j < W; ++j) p[j] = acc[j];
+      } else {
+        finish<TO, W>(a, key[u], col, acc);
+      }
+      from_before = false;
+#pragma unroll
+      for (int j = 0; j < W; ++j) acc[j] = 0.f;
+    }
+  }
+}
+
+template <typename TO, int W>
+__global__ void __launch_bounds__(SUM_NT) join_tokens_kernel(const Grad a) {
+  const int c = (int)blockIdx.x / a.col_tiles;
+  const int col = (((int)blockIdx.x % a.col_tiles) * SUM_NT + (int)threadIdx.x) * W;
+  const int total = a.start[a.V];
+  const int s1 = (c + 1) * a.chunk;  // the border behind this chunk
+  if (col >= a.d || s1 >= total) return;
+  const int id = a.key[s1 - 1];
+  if (a.key[s1] != id || a.start[id] < c * a.chunk) return;  // no run crosses it, or one that starts before
+  const int last = (a.start[id + 1] - 1) / a.chunk;          // the chunk in which it ends
+  float acc[W];
+  const float *p = a.part + ((int64_t)c * 2 + 1) * a.d + col;
+#pragma unroll
+  for (int j = 0; j < W; ++j) acc[j] = p[j];
+#pragma unroll 8
+  for (int k = c + 1; k <= last; ++k) {
+    const float *q = a.part + (int64_t)k * 2 * a.d + col;
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[j] += q[j];
+  }
+  finish<TO, W>(a, id, col, acc);
+}
+
+// ------------------------------------------------------------ host side
+
+static int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? MSTAR_OK : fail(MSTAR_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e));
+}
+
+static int check_dtype(int dtype, const char *what) {
+  if (dtype == MSTAR_DTYPE_F32 || dtype == MSTAR_DTYPE_BF16) return MSTAR_OK;
+  return fail(MSTAR_ERR_INVALID, std::string(what) + " must be MSTAR_DTYPE_F32 or MSTAR_DTYPE_BF16");
+}
+
+static int es(int dtype) { return dtype == MSTAR_DTYPE_F32 ? 4 : 2; }
+
+// Widest access that every row of a matrix allows: 8 values (16-byte
+// accesses), 2 (one access of a pair) or 1.
+static int width(const void *p, int64_t ld, int dtype) {
+  const uint64_t a = reinterpret_cast<uintptr_t>(p) | (uint64_t)ld * (uint64_t)es(dtype);
+  return a % 16 == 0 ? 8 : a % (2 * (uint64_t)es(dtype)) == 0 ? 2 : 1;
+}
+static int width_of(int d, int w) { return d % 8 == 0 && w == 8 ? 8 : d % 2 == 0 && w >= 2 ? 2 : 1; }
+
+static int check_lookup(const int64_t *ids, int64_t N, int V, int d, const void *out, int out_dtype) {
+  if (!ids || !out) return fail(MSTAR_ERR_INVALID, "ids and out must not be NULL");
+  if (N < 1 || N > (1 << 28)) return fail(MSTAR_ERR_INVALID, "N must be in [1, 2^28]");
+  if (V < 1 || V > (1 << 21)) return fail(MSTAR_ERR_INVALID, "V must be in [1, 2097152]");
+  if (d < 1 || d > (1 << 20)) return fail(MSTAR_ERR_INVALID, "d must be in [1, 2^20]");
+  int rc = check_dtype(out_dtype, "out_dtype");
+  if (rc) return rc;
+  if (reinterpret_cast<uintptr_t>(out) & (es(out_dtype) - 1))
+    return fail(MSTAR_ERR_INVALID, "out must be aligned to its type");
+  if ((N * d + NT * 4 - 1) / (NT * 4) > 0x7FFFFFFF) return fail(MSTAR_ERR_INVALID, "N * d is too large");
+  return MSTAR_OK;
+}
+
+template <typename TI, typename TO>
+static int launch_lookup(const Lookup &a, int w, cudaStream_t st) {
+  const unsigned grid = (unsigned)((a.N * (a.d / w) + NT * 4 - 1) / (NT * 4));
+  if (w == 8)
+    embed_kernel<TI, TO, 8><<<grid, NT, 0, st>>>(a);
+  else if (w == 2)
+    embed_kernel<TI, TO, 2><<<grid, NT, 0, st>>>(a);
+  else
+    embed_kernel<TI, TO, 1><<<grid, NT, 0, st>>>(a);
+  return launched();
+}
+
+// Workspace: start [V + 1], pos [N], key [N], part [nchunks][2][d], each
+// rounded to 256 bytes.
+struct Layout {
+  int chunk, nchunks, cols;
+  int64_t start, pos, key, part, bytes;
+};
+static Layout layout(int N, int V, int d) {
+  Layout l{};
+  // chunks long enough to amortise a border, short enough for some waves of CTAs
+  const int64_t tiles = (d + SUM_NT * 8 - 1) / (SUM_NT * 8);
+  l.chunk = (int)std::min<int64_t>(128, std::max<int64_t>(8, (int64_t)N * tiles / (148 * 8)));
+  l.nchunks = (N + l.chunk - 1) / l.chunk;
+  const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+  l.start = 0;
+  l.pos = up(((int64_t)V + 1) * 4);
+  l.key = l.pos + up((int64_t)N * 4);
+  l.part = l.key + up((int64_t)N * 4);
+  l.bytes = l.part + up((int64_t)l.nchunks * 2 * d * 4);
+  return l;
+}
+
+template <typename TI, typename TO, int W>
+static int launch_grad(Grad &a, cudaStream_t st) {
+  a.col_tiles = (a.d + SUM_NT * W - 1) / (SUM_NT * W);
+  const int grid = (a.V + a.bins - 1) / a.bins;
+  const int smem = SORT_NW * a.bins * 4;
+  cudaError_t e = cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+  sort_tokens_kernel<<<grid, SORT_NT, smem, st>>>(a);
+  int rc = launched();
+  if (rc) return rc;
+  const int64_t work = (int64_t)a.nchunks * a.col_tiles;
+  const bool in_place = a.base == a.out;
+  a.nzero = in_place ? 0 : (a.V + a.zero_rows - 1) / a.zero_rows;
+  sum_tokens_kernel<TI, TO, W><<<(unsigned)(work + a.nzero), SUM_NT, 0, st>>>(a);
+  if ((rc = launched())) return rc;
+  if (a.nchunks > 1) {
+    join_tokens_kernel<TO, W><<<(unsigned)work, SUM_NT, 0, st>>>(a);
+    rc = launched();
+  }
+  return rc;
+}
+
+template <typename TI, typename TO>
+static int launch_grad_w(Grad &a, int w, cudaStream_t st) {
+  return w == 8 ? launch_grad<TI, TO, 8>(a, st) : w == 2 ? launch_grad<TI, TO, 2>(a, st) : launch_grad<TI, TO, 1>(a, st);
+}
+
+}  // namespace emb
+}  // namespace mstar
+
+using namespace mstar;
+
+extern "C" {
+
+int mstar_embed_tokens(const int64_t *ids, int64_t N, const void *table, int32_t dtype, int32_t V, int32_t d,
+                       int64_t ld, float scale, void *out, int32_t out_dtype, uint32_t *status, void *stream) {
+  int rc = emb::check_lookup(ids, N, V, d, out, out_dtype);
+  if (rc) return rc;
+  if (!table) return fail(MSTAR_ERR_INVALID, "table must not be NULL");
+  if ((rc = emb::check_dtype(dtype, "dtype"))) return rc;
+  if (ld < d) return fail(MSTAR_ERR_INVALID, "ld must be >= d");
+  if (reinterpret_cast<uintptr_t>(table) & (emb::es(dtype) - 1))
+    return fail(MSTAR_ERR_INVALID, "table must be aligned to its type");
+  emb::Lookup a{};
+  a.table = table;
+  a.ld = ld;
+  a.ids = ids;
+  a.N = N;
+  a.V = V;
+  a.d = d;
+  a.scale = scale;
+  a.out = out;
+  a.status = status;
+  const int w = emb::width_of(d, std::min(emb::width(table, ld, dtype), emb::width(out, d, out_dtype)));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool fi = dtype == MSTAR_DTYPE_F32, fo = out_dtype == MSTAR_DTYPE_F32;
+  if (fi) return fo ? emb::launch_lookup<float, float>(a, w, st) : emb::launch_lookup<float, __nv_bfloat16>(a, w, st);
+  return fo ? emb::launch_lookup<__nv_bfloat16, float>(a, w, st)
+            : emb::launch_lookup<__nv_bfloat16, __nv_bfloat16>(a, w, st);
+}
+
+int mstar_embed_tokens_w4(const int64_t *ids, int64_t N, const mstar_w4_t *w, float scale, void *out,
+                          int32_t out_dtype, uint32_t *status, void *stream) {
+  int rc = check_w4(w);
+  if (rc) return rc;
+  if ((rc = emb::check_lookup(ids, N, w->V, w->d, out, out_dtype))) return rc;
+  if (reinterpret_cast<uintptr_t>(out) & 15u) return fail(MSTAR_ERR_INVALID, "out must be 16-byte aligned");
+  emb::Lookup a{};
+  a.ids = ids;
+  a.N = N;
+  a.V = w->V;
+  a.d = w->d;
+  a.scale = scale;
+  a.out = out;
+  a.status = status;
+  a.codes = static_cast<const uint8_t *>(w->codes);
+  a.scales = w->scales;
+  a.zeros = static_cast<const uint8_t *>(w->zeros);
+  a.scale_dtype = w->scale_dtype;
+  a.group_log2 = w->group == 32 ? 5 : w->group == 64 ? 6 : 7;
+  a.ngroups = w->d / w->group;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)((N * (w->d / 8) + emb::NT * 4 - 1) / (emb::NT * 4));
+  if (out_dtype == MSTAR_DTYPE_F32)
+    emb::embed_w4_kernel<float><<<grid, emb::NT, 0, st>>>(a);
+  else
+    emb::embed_w4_kernel<__nv_bfloat16><<<grid, emb::NT, 0, st>>>(a);
+  return emb::launched();
+}
+
+int64_t mstar_embed_grad_workspace_bytes(int32_t N, int32_t V, int32_t d) {
+  if (N < 1 || N > (1 << 24) || V < 1 || V > (1 << 21) || d < 1 || d > (1 << 16)) return -1;
+  return emb::layout(N, V, d).bytes;
+}
+
+int mstar_embed_tokens_grad(const int64_t *ids, int32_t N, const void *dout, int32_t dtype, int64_t ld, int32_t V,
+                            int32_t d, float scale, const void *base, void *out, int32_t out_dtype, void *workspace,
+                            int64_t workspace_bytes, uint32_t *status, void *stream) {
+  if (!ids || !dout || !out || !workspace)
+    return fail(MSTAR_ERR_INVALID, "ids, dout, out and workspace must not be NULL");
+  if (N < 1 || N > (1 << 24)) return fail(MSTAR_ERR_INVALID, "N must be in [1, 2^24]");
+  if (V < 1 || V > (1 << 21)) return fail(MSTAR_ERR_INVALID, "V must be in [1, 2097152]");
+  if (d < 1 || d > (1 << 16)) return fail(MSTAR_ERR_INVALID, "d must be in [1, 65536]");
+  int rc = emb::check_dtype(dtype, "dtype");
+  if (rc || (rc = emb::check_dtype(out_dtype, "out_dtype"))) return rc;
+  if (ld < d) return fail(MSTAR_ERR_INVALID, "ld must be >= d");
+  if (reinterpret_cast<uintptr_t>(dout) & (emb::es(dtype) - 1))
+    return fail(MSTAR_ERR_INVALID, "dout must be aligned to its type");
+  if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(base)) & (emb::es(out_dtype) - 1))
+    return fail(MSTAR_ERR_INVALID, "base and out must be aligned to their type");
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u)
+    return fail(MSTAR_ERR_INVALID, "workspace must be 256-byte aligned");
+  const emb::Layout l = emb::layout(N, V, d);
+  if (workspace_bytes < l.bytes) return fail(MSTAR_ERR_INVALID, "workspace too small");
+  uint8_t *ws = static_cast<uint8_t *>(workspace);
+  emb::Grad a{};
+  a.dout = dout;
+  a.ldo = ld;
+  a.ids = ids;
+  a.N = N;
+  a.V = V;
+  a.d = d;
+  a.scale = scale;
+  a.base = base;
+  a.out = out;
+  a.status = status;
+  // equal ranges, one per SM where the table allows it
+  a.bins = std::min(emb::MAX_BINS, (V + sm_count() - 1) / sm_count());
+  a.chunk = l.chunk;
+  a.nchunks = l.nchunks;
+  a.zero_rows = 8;
+  a.start = reinterpret_cast<int32_t *>(ws + l.start);
+  a.pos = reinterpret_cast<int32_t *>(ws + l.pos);
+  a.key = reinterpret_cast<int32_t *>(ws + l.key);
+  a.part = reinterpret_cast<float *>(ws + l.part);
+  int w = std::min(emb::width(dout, ld, dtype), emb::width(out, d, out_dtype));
+  if (base) w = std::min(w, emb::width(base, d, out_dtype));
+  w = emb::width_of(d, w);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool fi = dtype == MSTAR_DTYPE_F32, fo = out_dtype == MSTAR_DTYPE_F32;
+  if (fi)
+    return fo ? emb::launch_grad_w<float, float>(a, w, st) : emb::launch_grad_w<float, __nv_bfloat16>(a, w, st);
+  return fo ? emb::launch_grad_w<__nv_bfloat16, float>(a, w, st)
+            : emb::launch_grad_w<__nv_bfloat16, __nv_bfloat16>(a, w, st);
+}
+
+}  // extern "C"

@@ -363,3 +363,393 @@ def lmhead_step(hidden: torch.Tensor, weight: torch.Tensor, logits: torch.Tensor
                                                   _ptr(status), ctypes.c_void_p(stream)),
                 "mstar_sampler_lmhead_step")
     return p
+
+
+# ------------------------------------------------- 4-bit weights, lookup, log-probabilities, policy loss
+
+_ES = {torch.float32: 4, torch.bfloat16: 2}
+
+
+def _call(dev: torch.device, name: str, *args) -> None:
+    """Entry point `name` with `args` and the current stream of `dev`, on `dev`."""
+    fn = getattr(N.lib(), name)
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc != N.OK:
+        N.check(rc, name)
+
+
+def _cuda(t: torch.Tensor, name: str) -> torch.device:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    return t.device
+
+
+def _vec(t, name, dtype, dev, n):
+    """The address of a contiguous [n] tensor of `dtype` (None: NULL)."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != dev:
+        raise ValueError(f"{name} must live on {dev}, got {t.device}")
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{n}] tensor, got shape {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _status(t, dev):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.device != dev or t.numel() < 1:
+        raise ValueError(f"status must be an int32 tensor on {dev}")
+    return t.data_ptr()
+
+
+def _matrix(t, name, dev, rows, cols):
+    """Checks a [rows, cols] float32 / bfloat16 matrix with contiguous rows."""
+    if t.dtype not in _DT:
+        raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+    if t.device != dev:
+        raise ValueError(f"{name} must live on {dev}, got {t.device}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or (t.stride(1) != 1 and cols > 1):
+        raise ValueError(f"{name} must be [{rows}, {cols}] with contiguous rows, got shape {tuple(t.shape)} "
+                         f"with strides {t.stride()}")
+    if rows > 1 and t.stride(0) < cols:
+        raise ValueError(f"{name}'s rows overlap (row stride {t.stride(0)})")
+
+
+def _ld(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices' memory ranges meet without being the same rows."""
+    if a.data_ptr() == b.data_ptr() and _ld(a) == _ld(b) and a.dtype == b.dtype:
+        return False
+    span = lambda t: ((t.shape[0] - 1) * _ld(t) + t.shape[1]) * _ES[t.dtype]  # noqa: E731
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    return a0 < b0 + span(b) and b0 < a0 + span(a)
+
+
+def quantize_w4(weight: torch.Tensor, group_size: int = 128, *, zero_points: bool = False, scale_dtype=torch.bfloat16):
+    """Round a [V, d] weight to 4 bits with one scale per row and group of
+    `group_size` columns: (codes [V, d / 2] uint8, the even column in the low
+    four bits; scales [V, d / group_size]; zeros uint8 or None).  Without zero
+    points codes run from -8 to 7 about 8; with them each group's range maps
+    to 0 .. 15.  A one-time step on any device (plain tensor operations)."""
+    if weight.dim() != 2:
+        raise ValueError("weight must be [V, d]")
+    if group_size not in (32, 64, 128) or weight.shape[1] % group_size:
+        raise ValueError("group_size must be 32, 64 or 128 and divide d")
+    if scale_dtype not in _DT:
+        raise TypeError("scale_dtype must be float32 or bfloat16")
+    V, d = weight.shape
+    w = weight.detach().float().view(V, d // group_size, group_size)
+    if zero_points:
+        lo, hi = w.amin(2).clamp(max=0), w.amax(2).clamp(min=0)
+        scales = ((hi - lo) / 15).to(scale_dtype)
+    else:
+        scales = (w.abs().amax(2) / 7.5).to(scale_dtype)
+    s = scales.float()
+    s = torch.where(s > 0, s, 1.0)
+    zeros = (-lo / s).round().clamp(0, 15) if zero_points else torch.full_like(s, 8.0)
+    q = (w / s[:, :, None] + zeros[:, :, None]).round().clamp(0, 15).to(torch.uint8).view(V, d)
+    return q[:, 0::2] | (q[:, 1::2] << 4), scales, zeros.to(torch.uint8) if zero_points else None
+
+
+def _w4(codes, scales, zeros) -> N.W4:
+    dev = _cuda(codes, "codes")
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous():
+        raise ValueError("codes must be a contiguous [V, d / 2] uint8 tensor")
+    if scales.dtype not in _DT:
+        raise TypeError(f"scales must be float32 or bfloat16, got {scales.dtype}")
+    V, d = codes.shape[0], codes.shape[1] * 2
+    if scales.device != dev or scales.dim() != 2 or scales.shape[0] != V or not scales.is_contiguous():
+        raise ValueError("scales must be a contiguous [V, d / group] tensor on the codes' device")
+    G = scales.shape[1]
+    if G < 1 or d % G or d // G not in (32, 64, 128):
+        raise ValueError(f"scales give groups of {d / max(G, 1):g} columns; they must be of 32, 64 or 128")
+    w = N.W4()
+    if zeros is not None:
+        if zeros.dtype != torch.uint8 or zeros.device != dev or zeros.shape != scales.shape or not zeros.is_contiguous():
+            raise ValueError("zeros must be a contiguous uint8 tensor of the scales' shape on their device")
+        w.zeros = zeros.data_ptr()
+    w.codes, w.scales = codes.data_ptr(), scales.data_ptr()
+    w.V, w.d, w.group, w.scale_dtype = V, d, d // G, _DT[scales.dtype]
+    return w
+
+
+def _check_hidden_w4(hidden, w, dev):
+    if hidden.dtype != torch.bfloat16:
+        raise TypeError(f"hidden must be bfloat16, got {hidden.dtype}")
+    _matrix(hidden, "hidden", dev, hidden.shape[0], w.d)
+    B = hidden.shape[0]
+    if not 1 <= B <= 256:
+        raise ValueError(f"B={B} is outside [1, 256]")
+    return B
+
+
+def lmhead_w4_workspace(B: int, V: int, d: int, device) -> torch.Tensor:
+    """Scratch for lmhead_logits_w4 calls of these sizes
+    (mstar_lmhead_w4_workspace_bytes); calls that share it must not overlap."""
+    dev = torch.device(device)
+    with torch.cuda.device(dev):
+        n = int(N.lib().mstar_lmhead_w4_workspace_bytes(B, V, d))
+    if n <= 0:
+        N.check(N.ERR_INVALID, "mstar_lmhead_w4_workspace_bytes")
+    return torch.empty(n, dtype=torch.uint8, device=dev)
+
+
+def lmhead_logits_w4(hidden: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, zeros=None,
+                     out: torch.Tensor | None = None, dtype=torch.float32, status: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """hidden [B, d] (bfloat16, any row stride) times a 4-bit weight [V, d]
+    transposed (mstar_lmhead_logits_w4): (code - zero) * scale, codes
+    [V, d / 2] uint8 with the even column in the low four bits, scales
+    [V, d / group] float32 or bfloat16, zeros uint8 of the same shape or None
+    for 8.  fp32 sums, stored as float32 or bfloat16.  workspace: None takes
+    fresh scratch from torch's allocator (safe on any stream and inside graph
+    capture), or pass lmhead_w4_workspace's."""
+    w = _w4(codes, scales, zeros)
+    dev = codes.device
+    B = _check_hidden_w4(hidden, w, dev)
+    if out is None:
+        out = torch.empty(B, w.V, dtype=dtype, device=dev)
+    else:
+        _matrix(out, "out", dev, B, w.V)
+    if workspace is None:
+        workspace = lmhead_w4_workspace(B, w.V, w.d, dev)
+    wp, wn = _check_ws(workspace, dev)
+    _call(dev, "mstar_lmhead_logits_w4", hidden.data_ptr(), _ld(hidden), B, ctypes.byref(w), out.data_ptr(),
+          _DT[out.dtype], _ld(out), wp, wn, _status(status, dev))
+    return out
+
+
+def lmhead_step_w4(hidden: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, logits: torch.Tensor, *,
+                   zeros=None, status=None, workspace: torch.Tensor | None = None, **kw) -> N.Params:
+    """lmhead_logits_w4 into `logits` [B, V] (written) and one sampling step
+    on it (mstar_sampler_lmhead_step_w4).  The sampling keywords are
+    sampler_step's; the logits are read back from L2."""
+    w = _w4(codes, scales, zeros)
+    dev = codes.device
+    B = _check_hidden_w4(hidden, w, dev)
+    _matrix(logits, "logits", dev, B, w.V)
+    p = build_params(logits, **kw)
+    if workspace is None:
+        workspace = lmhead_w4_workspace(B, w.V, w.d, dev)
+    wp, wn = _check_ws(workspace, dev)
+    _call(dev, "mstar_sampler_lmhead_step_w4", ctypes.byref(p), hidden.data_ptr(), _ld(hidden), ctypes.byref(w), wp,
+          wn, _status(status, dev))
+    return p
+
+
+def _ids_1d(ids, dev):
+    if ids.dtype != torch.int64:
+        raise TypeError(f"ids must be int64, got {ids.dtype}")
+    if ids.device != dev:
+        raise ValueError(f"ids must live on {dev}, got {ids.device}")
+    if not ids.is_contiguous():
+        raise ValueError("ids must be contiguous")
+    return ids.numel()
+
+
+def _lookup_out(ids, d, out, dtype, dev):
+    if out is None:
+        if dtype not in _DT:
+            raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
+        return torch.empty(*ids.shape, d, dtype=dtype, device=dev)
+    if out.dtype not in _DT:
+        raise TypeError(f"out must be float32 or bfloat16, got {out.dtype}")
+    if out.device != dev or out.shape != (*ids.shape, d) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {(*ids.shape, d)} tensor on {dev}")
+    return out
+
+
+def embed_tokens(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out: torch.Tensor | None = None,
+                 dtype=None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """scale * table[ids] (mstar_embed_tokens): ids int64 of any shape, table
+    [V, d] float32 or bfloat16 with contiguous rows; the result is ids.shape +
+    (d,) of `dtype` (the table's by default).  The product is made in float32
+    and rounded once.  A negative id gives zeros (a padding row); an id >= V
+    does too and sets STATUS_BAD_ID in `status`."""
+    dev = _cuda(table, "table")
+    if table.dim() != 2:
+        raise ValueError("table must be [V, d]")
+    V, d = table.shape
+    _matrix(table, "table", dev, V, d)
+    n = _ids_1d(ids, dev)
+    out = _lookup_out(ids, d, out, dtype or table.dtype, dev)
+    st = _status(status, dev)
+    if n:
+        _call(dev, "mstar_embed_tokens", ids.data_ptr(), n, table.data_ptr(), _DT[table.dtype], V, d, _ld(table),
+              scale, out.data_ptr(), _DT[out.dtype], st)
+    return out
+
+
+def embed_tokens_w4(ids: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, zeros=None, scale: float = 1.0,
+                    out: torch.Tensor | None = None, dtype=torch.bfloat16,
+                    status: torch.Tensor | None = None) -> torch.Tensor:
+    """embed_tokens from a 4-bit table (mstar_embed_tokens_w4), the tied
+    weight of lmhead_logits_w4: scale * (code - zero) * group scale."""
+    w = _w4(codes, scales, zeros)
+    dev = codes.device
+    n = _ids_1d(ids, dev)
+    out = _lookup_out(ids, w.d, out, dtype, dev)
+    st = _status(status, dev)
+    if n:
+        _call(dev, "mstar_embed_tokens_w4", ids.data_ptr(), n, ctypes.byref(w), scale, out.data_ptr(), _DT[out.dtype],
+              st)
+    return out
+
+
+def embed_tokens_grad(ids: torch.Tensor, dout: torch.Tensor, V: int, *, scale: float = 1.0,
+                      base: torch.Tensor | None = None, out: torch.Tensor | None = None, dtype=None,
+                      status: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of embed_tokens to its [V, d] table
+    (mstar_embed_tokens_grad): base + scale * (the sum of dout's rows over the
+    positions of each id), every row written.  dout is [N, d] (float32 or
+    bfloat16, contiguous rows) for ids of N elements; base (None: zeros) has
+    the result's type and may be `out` itself, which adds in place (the tied
+    head's gradient, or an earlier micro-batch's).  Sums are float32 in
+    position order, so equal inputs give equal bits; rounded once."""
+    dev = _cuda(dout, "dout")
+    n = _ids_1d(ids, dev)
+    if dout.dim() != 2:
+        raise ValueError("dout must be [N, d]")
+    d = dout.shape[1]
+    _matrix(dout, "dout", dev, n, d)
+    if V < 1:
+        raise ValueError("V must be >= 1")
+    if out is None:
+        out = torch.empty(V, d, dtype=dtype or (dout.dtype if base is None else base.dtype), device=dev)
+    if base is not None:
+        if base.dtype != out.dtype:
+            raise TypeError(f"base must have out's type {out.dtype}, got {base.dtype}")
+        _matrix(base, "base", dev, V, d)
+        if not base.is_contiguous() or _overlap(base, out):
+            raise ValueError("base must be contiguous, and out itself or apart from it")
+    _matrix(out, "out", dev, V, d)
+    if not out.is_contiguous():
+        raise ValueError("out must be contiguous")
+    if _overlap(dout, out) or out.data_ptr() == dout.data_ptr():
+        raise ValueError("out must not overlap dout")
+    st = _status(status, dev)
+    if n == 0:
+        if base is None:
+            return out.zero_()
+        return out if base.data_ptr() == out.data_ptr() else out.copy_(base)
+    nbytes = int(N.lib().mstar_embed_grad_workspace_bytes(n, V, d))
+    if nbytes <= 0:
+        raise ValueError(f"N={n}, V={V}, d={d} are outside [1, 2^24], [1, 2^21], [1, 65536]")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call(dev, "mstar_embed_tokens_grad", ids.data_ptr(), n, dout.data_ptr(), _DT[dout.dtype], _ld(dout), V, d, scale,
+          None if base is None else base.data_ptr(), out.data_ptr(), _DT[out.dtype], ws.data_ptr(), nbytes, st)
+    return out
+
+
+def _check_rows(logits, ids, temperature):
+    dev = _cuda(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError("logits must be [N, V]")
+    n, V = logits.shape
+    _matrix(logits, "logits", dev, n, V)
+    ip = _vec(ids, "ids", torch.int64, dev, n)
+    if not 1e-5 <= temperature <= 1e5:
+        raise ValueError(f"temperature must be in [1e-5, 1e5], got {temperature}")
+    return dev, n, V, ip
+
+
+def _grad_out(out, logits, dev, n, V, name):
+    if out is None:
+        return torch.empty(n, V, dtype=logits.dtype, device=dev)
+    _matrix(out, name, dev, n, V)
+    if out.dtype != logits.dtype:
+        raise TypeError(f"{name} must have the logits' type {logits.dtype}, got {out.dtype}")
+    if _overlap(out, logits):
+        raise ValueError(f"{name} must be the logits themselves or apart from them")
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, temperature: float = 1.0,
+                   logp: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                   status: torch.Tensor | None = None):
+    """(logp [N], lse [N]) float32 of ids [N] under softmax(logits /
+    temperature), logits [N, V] float32 or bfloat16 (mstar_token_logprobs).
+    -inf logits are masked ids; a row of nothing else gives -inf and
+    STATUS_EMPTY.  A negative id is a padding row (logp 0); an id >= V counts
+    as one and sets STATUS_BAD_ID."""
+    dev, n, V, ip = _check_rows(logits, ids, temperature)
+    if logp is None:
+        logp = torch.empty(n, dtype=torch.float32, device=dev)
+    if lse is None:
+        lse = torch.empty(n, dtype=torch.float32, device=dev)
+    lp, ls, st = _vec(logp, "logp", torch.float32, dev, n), _vec(lse, "lse", torch.float32, dev, n), _status(status, dev)
+    if n:
+        _call(dev, "mstar_token_logprobs", logits.data_ptr(), _DT[logits.dtype], n, V, _ld(logits), ip, temperature,
+              lp, ls, st)
+    return logp, lse
+
+
+def token_logprobs_grad(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor, dlogp: torch.Tensor, *,
+                        temperature: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of sum(dlogp * logp) to the logits, of their type
+    (mstar_token_logprobs_grad); lse is token_logprobs'.  out may be the
+    logits themselves (replaced in place).  Padding and empty rows: zeros."""
+    dev, n, V, ip = _check_rows(logits, ids, temperature)
+    lp, dp = _vec(lse, "lse", torch.float32, dev, n), _vec(dlogp, "dlogp", torch.float32, dev, n)
+    out = _grad_out(out, logits, dev, n, V, "out")
+    if n:
+        _call(dev, "mstar_token_logprobs_grad", logits.data_ptr(), _DT[logits.dtype], n, V, _ld(logits), ip,
+              temperature, lp, dp, out.data_ptr(), _ld(out))
+    return out
+
+
+def policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logp: torch.Tensor | None, advantages: torch.Tensor, *,
+                ref_logp: torch.Tensor | None = None, weights: torch.Tensor | None = None, temperature: float = 1.0,
+                clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, grad: bool = True,
+                loss: torch.Tensor | None = None, logp: torch.Tensor | None = None,
+                dlogits: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """Clipped policy loss per token and its gradient in one pass over the
+    logits (mstar_policy_loss): (loss [N], logp [N], dlogits [N, V] or None).
+
+        r = exp(logp - old_logp)           (old_logp None: on policy, r = 1)
+        loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+               + kl_coef (exp(ref_logp - logp) - (ref_logp - logp) - 1)
+        dlogits = the gradient of sum(weights * loss), weights None: 1
+
+    logits [N, V] float32 or bfloat16; the per-token tensors are float32 [N].
+    dlogits has the logits' type; give the logits themselves to replace them
+    in place, or grad=False for the values alone.  A negative id is a padding
+    row: loss 0, logp 0, a zero gradient, and its logits are not read."""
+    dev, n, V, ip = _check_rows(logits, ids, temperature)
+    f32 = torch.float32
+    p = N.PolicyParams()
+    p.ids = ip
+    p.old_logp = _vec(old_logp, "old_logp", f32, dev, n)
+    p.ref_logp = _vec(ref_logp, "ref_logp", f32, dev, n)
+    p.advantages = _vec(advantages, "advantages", f32, dev, n)
+    p.weights = _vec(weights, "weights", f32, dev, n)
+    if not (0 <= clip_low <= 1 and clip_high >= 0 and kl_coef >= 0):
+        raise ValueError("clip_low must be in [0, 1], clip_high and kl_coef >= 0")
+    if kl_coef > 0 and ref_logp is None:
+        raise ValueError("kl_coef needs ref_logp")
+    if dlogits is not None and not grad:
+        raise ValueError("dlogits is given, but grad is False")
+    if loss is None:
+        loss = torch.empty(n, dtype=f32, device=dev)
+    if logp is None:
+        logp = torch.empty(n, dtype=f32, device=dev)
+    p.loss, p.logp = _vec(loss, "loss", f32, dev, n), _vec(logp, "logp", f32, dev, n)
+    if grad:
+        dlogits = _grad_out(dlogits, logits, dev, n, V, "dlogits")
+        p.dlogits, p.ld_dlogits = dlogits.data_ptr(), _ld(dlogits)
+    p.logits, p.dtype, p.N, p.V, p.ld = logits.data_ptr(), _DT[logits.dtype], n, V, _ld(logits)
+    p.temperature, p.clip_low, p.clip_high, p.kl_coef = temperature, clip_low, clip_high, kl_coef
+    p.status = _status(status, dev)
+    if n:
+        _call(dev, "mstar_policy_loss", ctypes.byref(p))
+    return loss, logp, dlogits

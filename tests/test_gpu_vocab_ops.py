@@ -1,0 +1,493 @@
+"""GPU: the 4-bit LM head, the embedding lookup and its gradient, token
+log-probabilities and the policy loss, against their 64-bit definitions with
+tolerances counted from the roundings (tests/vocab_ref.py)."""
+import math
+
+import pytest
+import torch
+
+from tests import vocab_ref as R
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def near(got, ref, tol):
+    bad = ~((got.double() - ref).abs() <= tol)
+    assert not bool(bad.any()), (int(bad.sum()), float(((got.double() - ref).abs() / tol)[bad].max()),
+                                 bad.nonzero()[:3].tolist())
+
+
+def w4_inputs(V, d, g, stype, zeros, seed):
+    G = gen(seed)
+    codes = torch.randint(0, 256, (V, d // 2), device="cuda", dtype=torch.uint8, generator=G)
+    scales = ((torch.rand(V, d // g, device="cuda", generator=G) + 0.3) / math.sqrt(d)).to(stype)
+    z = torch.randint(0, 16, (V, d // g), device="cuda", dtype=torch.uint8, generator=G) if zeros else None
+    return codes, scales, z
+
+
+W4_CASES = [
+    # B, V, d, group, scale type, zero points, output type
+    (1, 1, 32, 32, F32, False, F32),             # the smallest call
+    (1, 1000, 256, 128, BF16, False, F32),
+    (2, 257, 128, 128, BF16, True, BF16),        # one row past a tile; one block
+    (16, 4099, 1024, 32, F32, True, F32),        # codec head, fine groups
+    (17, 2049, 96, 32, BF16, False, BF16),       # d inside one block
+    (33, 1500, 416, 32, F32, True, F32),         # d = 3 blocks and a group
+    (48, 777, 1600, 64, BF16, False, F32),       # columns beyond the MMA's N
+    (64, 20000, 2048, 128, BF16, True, BF16),
+    (65, 515, 192, 64, F32, False, F32),         # last stage of one block
+    (100, 3001, 4096, 64, BF16, True, F32),
+    (128, 5000, 640, 128, F32, False, BF16),
+    (129, 1111, 512, 32, BF16, True, F32),       # two chunks of rows
+    (200, 2500, 1024, 64, BF16, False, BF16),
+    (256, 900, 2048, 128, F32, True, F32),
+]
+
+
+@pytest.mark.parametrize("B,V,d,g,stype,zeros,odt", W4_CASES)
+def test_lmhead_w4(B, V, d, g, stype, zeros, odt):
+    from mstar_rs_b200 import kernel
+
+    codes, scales, z = w4_inputs(V, d, g, stype, zeros, B + V + d)
+    hidden = torch.randn(B, d, device="cuda", generator=gen(d)).to(BF16)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = kernel.lmhead_logits_w4(hidden, codes, scales, zeros=z, dtype=odt, status=status)
+    again = kernel.lmhead_logits_w4(hidden, codes, scales, zeros=z, dtype=odt, status=status)
+    ref, tol = R.head(hidden, codes, scales, z, odt, parts=16)
+    near(out, ref, tol + 1e-30)
+    assert torch.equal(out, again)
+    assert status.item() == 0
+
+
+def test_lmhead_w4_strided_rows():
+    """Hidden rows with a stride and an odd start, logits inside a wider
+    buffer: only [:, :V] is written."""
+    from mstar_rs_b200 import kernel
+
+    B, V, d = 5, 1001, 256
+    codes, scales, z = w4_inputs(V, d, 64, BF16, True, 3)
+    wide = torch.randn(B, d + 33, device="cuda", generator=gen(1)).to(BF16)
+    hidden = wide[:, 3:3 + d]
+    buf = torch.full((B, V + 23), 7.0, device="cuda")
+    kernel.lmhead_logits_w4(hidden, codes, scales, zeros=z, out=buf[:, 1:1 + V])
+    ref, tol = R.head(hidden, codes, scales, z, F32, parts=16)
+    near(buf[:, 1:1 + V], ref, tol)
+    assert bool((buf[:, :1] == 7).all()) and bool((buf[:, 1 + V:] == 7).all())
+
+
+def test_lmhead_w4_zero_scales_and_extremes():
+    """Zero scales give zeros; every code at its zero point too; large hidden
+    values pass through exactly."""
+    from mstar_rs_b200 import kernel
+
+    V, d = 300, 128
+    codes = torch.full((V, d // 2), 0x88, device="cuda", dtype=torch.uint8)
+    codes[1] = 0x0F  # even columns 15, odd 0
+    scales = torch.ones(V, 1, device="cuda")
+    scales[2] = 0.0
+    codes[2] = 0xFF
+    hidden = torch.full((2, d), 2.0 ** 100, device="cuda").to(BF16)
+    hidden[1] = -(2.0 ** -100)
+    out = kernel.lmhead_logits_w4(hidden, codes, scales)
+    want = torch.zeros(2, V, device="cuda")
+    want[0, 1], want[1, 1] = (7 - 8) * 64 * 2.0 ** 100, -(7 - 8) * 64 * 2.0 ** -100
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("B,V,d,dtype", [(64, 151936, 2048, "bf16"), (1, 156940, 1024, "f32"), (24, 32000, 512, "bf16"),
+                                         (130, 4096, 256, "f32")])
+def test_lmhead_step_w4_matches_the_two_calls(B, V, d, dtype):
+    from mstar_rs_b200 import kernel
+    from mstar_rs_b200 import workloads as W
+
+    case = W.qwen_mixed(seed=5, B=B, V=V)
+    case.dtype = dtype
+    kw = W.to_device(case)
+    kw.pop("logits")
+    codes, scales, z = w4_inputs(V, d, 128, BF16, True, 9)
+    hidden = torch.randn(B, d, device="cuda", generator=gen(4)).to(BF16)
+    tdt = BF16 if dtype == "bf16" else F32
+    logits = torch.empty(B, V, dtype=tdt, device="cuda")
+    ids, ids2 = (torch.zeros(B, dtype=torch.int64, device="cuda") for _ in range(2))
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kernel.lmhead_step_w4(hidden, codes, scales, logits, zeros=z, status=st, **kw, out_ids=ids)
+    ref = kernel.lmhead_logits_w4(hidden, codes, scales, zeros=z, dtype=tdt)
+    kernel.sampler_step(ref, **kw, out_ids=ids2)
+    assert torch.equal(logits, ref) and torch.equal(ids, ids2)
+    assert st.item() == 0
+
+
+# ------------------------------------------------------------ lookup
+
+
+@pytest.mark.parametrize("shape,V,d,tt,ot", [
+    ((1,), 1, 1, F32, F32), ((64,), 1000, 2048, BF16, BF16), ((3, 7), 100, 501, BF16, F32),
+    ((1000,), 333, 96, F32, BF16), ((5,), 50, 34, BF16, BF16), ((77,), 4099, 1023, F32, F32),
+    ((0,), 10, 8, BF16, BF16), ((2, 0, 3), 10, 8, F32, F32)])
+def test_embed(shape, V, d, tt, ot):
+    from mstar_rs_b200 import kernel
+
+    table = torch.randn(V, d, device="cuda", generator=gen(d)).to(tt)
+    ids = torch.randint(-2, V, shape, device="cuda", generator=gen(V))
+    out = kernel.embed_tokens(ids, table, scale=math.sqrt(d), dtype=ot)
+    assert out.shape == (*shape, d) and out.dtype == ot
+    ref = torch.where((ids < 0)[..., None], 0.0, table.double()[ids.clamp(min=0)] * math.sqrt(d))
+    near(out, ref, ref.abs() * (R.HALF[ot] + 2.0 ** -23))  # sqrt(d) as a float, the product, the rounding
+
+
+def test_embed_strided_table_and_bad_ids():
+    from mstar_rs_b200 import _native as N
+    from mstar_rs_b200 import kernel
+
+    wide = torch.randn(50, 75, device="cuda", generator=gen(2)).to(BF16)
+    table = wide[:, 3:67]  # 64 columns, odd start and stride
+    ids = torch.tensor([0, 49, 50, -1, 2 ** 40, -2 ** 62, 7], device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = kernel.embed_tokens(ids, table, status=status)
+    want = torch.zeros(7, 64, device="cuda", dtype=BF16)
+    want[[0, 1, 6]] = table[[0, 49, 7]]
+    assert torch.equal(out, want)
+    assert status.item() == N.STATUS_BAD_ID
+    status.zero_()
+    kernel.embed_tokens(ids[[0, 1, 3]].contiguous(), table, status=status)
+    assert status.item() == 0  # padding is no error
+
+
+@pytest.mark.parametrize("N_,V,d,g,st,z,ot", [(1, 1, 32, 32, F32, False, F32), (64, 999, 2048, 128, BF16, True, BF16),
+                                              (333, 77, 192, 64, BF16, False, F32), (9, 5, 416, 32, F32, True, BF16)])
+def test_embed_w4(N_, V, d, g, st, z, ot):
+    from mstar_rs_b200 import kernel
+
+    codes, scales, zeros = w4_inputs(V, d, g, st, z, N_)
+    ids = torch.randint(-1, V + 1, (N_,), device="cuda", generator=gen(5))
+    out = kernel.embed_tokens_w4(ids, codes, scales, zeros=zeros, scale=1.7, dtype=ot)
+    ok = (ids >= 0) & (ids < V)
+    ref = torch.where(ok[:, None], R.dequant(codes, scales, zeros)[ids.clamp(0, V - 1)] * 1.7, 0.0)
+    near(out, ref, ref.abs() * (R.HALF[ot] + 3 * 2.0 ** -24))
+
+
+GRAD_CASES = [
+    # N, V, d, type, output type, ids
+    (1, 1, 1, F32, F32, "all"), (5, 7, 3, BF16, BF16, "all"), (1000, 50, 64, BF16, F32, "all"),
+    (3000, 151936, 128, BF16, BF16, "zipf"), (4097, 3, 130, F32, F32, "all"),        # runs over many chunks
+    (2048, 5000, 2048, BF16, BF16, "one"),                                           # every token the same id
+    (2049, 1200, 501, BF16, F32, "zipf"), (777, 300, 1026, F32, BF16, "ends"), (100, 40, 256, BF16, F32, "none"),
+    (20000, 200000, 24, F32, F32, "zipf"),                                           # more ranges than SMs
+]
+
+
+@pytest.mark.parametrize("base", ["none", "apart", "in place"])
+@pytest.mark.parametrize("N_,V,d,tt,ot,kind", GRAD_CASES)
+def test_embed_grad(N_, V, d, tt, ot, kind, base):
+    from mstar_rs_b200 import kernel
+
+    G = gen(N_ + V)
+    if kind == "all":
+        ids = torch.randint(-1, V, (N_,), device="cuda", generator=G)
+    elif kind == "zipf":
+        u = torch.rand(N_, device="cuda", generator=G, dtype=torch.float64)
+        ids = (torch.exp(u * math.log(V + 1)).long() - 1).clamp(0, V - 1)
+    elif kind == "one":
+        ids = torch.full((N_,), V - 1, device="cuda")
+    elif kind == "ends":
+        ids = torch.where(torch.rand(N_, device="cuda", generator=G) < 0.5, 0, V - 1)
+    else:
+        ids = torch.full((N_,), -1, device="cuda")
+    dout = torch.randn(N_, d, device="cuda", generator=G).to(tt)
+    b = None if base == "none" else torch.randn(V, d, device="cuda", generator=G).to(ot)
+    ref, tol = R.embed_grad(ids, dout, V, 0.37, b, ot)
+    tol = tol + ref.abs() * 2.0 ** -23  # 0.37 as a float
+    keep = None if b is None else b.clone()
+    out = kernel.embed_tokens_grad(ids, dout, V, scale=0.37, base=b, out=b if base == "in place" else None, dtype=ot)
+    assert out.dtype == ot and out.shape == (V, d)
+    near(out, ref, tol)
+    if base == "apart":
+        assert torch.equal(b, keep)
+    if base != "in place":
+        assert torch.equal(out, kernel.embed_tokens_grad(ids, dout, V, scale=0.37, base=b, dtype=ot))
+
+
+def test_embed_grad_by_differences():
+    """The lookup is linear, so its gradient applied to a change of the table
+    is the change of sum(dout * lookup), up to the sums' roundings."""
+    from mstar_rs_b200 import kernel
+
+    V, d, n = 40, 24, 300
+    G = gen(8)
+    ids = torch.randint(-1, V, (n,), device="cuda", generator=G)
+    dout = torch.randn(n, d, device="cuda", generator=G)
+    step = torch.randn(V, d, device="cuda", generator=G)
+    grad = kernel.embed_tokens_grad(ids, dout, V, scale=3.0)
+    moved = kernel.embed_tokens(ids, step, scale=3.0)
+    a = (moved.double() * dout.double()).sum()
+    b = (grad.double() * step.double()).sum()
+    size = (moved.double().abs() * dout.double().abs()).sum()
+    assert abs(a - b) <= size * (n + 3) * 2.0 ** -24
+
+
+def test_embed_grad_strided_and_bad_ids():
+    from mstar_rs_b200 import _native as N
+    from mstar_rs_b200 import kernel
+
+    wide = torch.randn(200, 77, device="cuda", generator=gen(3)).to(BF16)
+    dout = wide[:, 5:70]
+    ids = torch.randint(0, 30, (200,), device="cuda", generator=gen(4))
+    ids[::7], ids[3], ids[10] = -5, 30, 2 ** 33 + 1
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = kernel.embed_tokens_grad(ids, dout, 30, status=status, dtype=F32)
+    ref, tol = R.embed_grad(ids, dout, 30, 1.0, None, F32)
+    near(out, ref, tol)
+    assert status.item() == N.STATUS_BAD_ID
+
+
+# ------------------------------------------------------------ log-probabilities and the policy loss
+
+
+def row_inputs(n, V, dtype, seed, masked=0.0):
+    G = gen(seed)
+    x = torch.randn(n, V, device="cuda", generator=G) * 3
+    ids = torch.randint(0, V, (n,), device="cuda", generator=G)
+    if masked:
+        x.masked_fill_(torch.rand(n, V, device="cuda", generator=G) < masked, -math.inf)
+        x[torch.arange(n), ids] = 1.0
+    if n > 3:
+        ids[1], ids[3] = -1, V  # padding, and a bad id
+    return x.to(dtype), ids
+
+
+ROW_CASES = [(1, 1, F32), (1, 2, BF16), (5, 7, BF16), (64, 1000, BF16), (3, 32001, F32), (7, 151936, BF16),
+             (2, 257152, F32), (300, 4097, F32), (1000, 128, BF16), (2, 600001, BF16), (1, 1000000, F32)]
+
+
+@pytest.mark.parametrize("T", [1.0, 0.37])
+@pytest.mark.parametrize("n,V,dtype", ROW_CASES)
+def test_token_logprobs_and_gradient(n, V, dtype, T):
+    from mstar_rs_b200 import kernel
+
+    x, ids = row_inputs(n, V, dtype, n + V, masked=0.3 if V > 100 else 0.0)
+    logp, lse = kernel.token_logprobs(x, ids, temperature=T)
+    valid, rl, rp = R.rows(x, ids, T)
+    near(lse, rl, R.SUM + rl.abs() * 2.0 ** -23)
+    near(logp, rp, torch.where(valid, R.SUM + rp.abs() * 2.0 ** -23, 0.0))
+    dlogp = torch.randn(n, device="cuda", generator=gen(1))
+    out = kernel.token_logprobs_grad(x, ids, lse, dlogp, temperature=T)
+    # the given lse, rounded to 32 bits, is the definition's here
+    ref, tol = R.grad(x, ids, T, lse.double(), dlogp.double(), dtype, rel=2.0 ** -20)
+    near(out, ref, tol)
+    same = kernel.token_logprobs_grad(x, ids, lse, dlogp, temperature=T, out=x)  # in place
+    assert same is x and torch.equal(x, out)
+
+
+@pytest.mark.parametrize("n,V,dtype", ROW_CASES)
+@pytest.mark.parametrize("old,ref,T", [(True, True, 1.0), (True, False, 0.6), (False, True, 1.7)])
+def test_policy_loss(n, V, dtype, old, ref, T):
+    from mstar_rs_b200 import kernel
+
+    x, ids = row_inputs(n, V, dtype, n * 3 + V, masked=0.3 if V > 100 else 0.0)
+    G = gen(7)
+    _, _, lp = R.rows(x, ids, T)
+    noise = torch.randn(n, device="cuda", generator=G, dtype=torch.float64) * 0.2
+    r = noise.exp()
+    noise += 0.02 * (((r - 0.9).abs() < 5e-3) | ((r - 1.3).abs() < 5e-3))  # off the border, where the gradient jumps
+    olp = (lp - noise).float() if old else None
+    rlp = (lp + 0.5 * torch.randn(n, device="cuda", generator=G)).float() if ref else None
+    adv = torch.randn(n, device="cuda", generator=G)
+    w = torch.rand(n, device="cuda", generator=G)
+    beta = 0.1 if ref else 0.0
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kw = dict(ref_logp=rlp, weights=w, temperature=T, clip_low=0.1, clip_high=0.3, kl_coef=beta, status=status)
+    loss, logp, dx = kernel.policy_loss(x, ids, olp, adv, **kw)
+    rloss, ltol, rlp_, d, dtol, lse = R.policy(x, ids, olp, adv, T, 0.1, 0.3, beta, rlp, w)
+    near(loss, rloss, ltol)
+    near(logp, rlp_, torch.where(R.rows(x, ids, T)[0], R.SUM + rlp_.abs() * 2.0 ** -23, 0.0))
+    gref, gtol = R.grad(x, ids, T, lse, d, dtype)
+    near(dx, gref, gtol + (dtol / T)[:, None] * 2)
+    assert status.item() == (0x80 if n > 3 else 0)
+    loss2, logp2, none = kernel.policy_loss(x, ids, olp, adv, **kw, grad=False)
+    assert none is None and torch.equal(loss2, loss) and torch.equal(logp2, logp)
+    _, _, same = kernel.policy_loss(x, ids, olp, adv, **kw, dlogits=x)  # in place
+    assert same is x and torch.equal(x, dx)
+
+
+def test_policy_gradient_by_differences():
+    """(loss(x + h u) - loss(x - h u)) / 2h along random directions, in f32
+    logits, against the gradient: within the third-order term (h^2 |u|^3-ish,
+    h = 1e-2 on unit directions: under 1e-3 of the gradient's size) and the
+    loss's own rounding over 2h."""
+    from mstar_rs_b200 import kernel
+
+    n, V = 6, 50
+    G = gen(11)
+    x = torch.randn(n, V, device="cuda", generator=G)
+    ids = torch.randint(0, V, (n,), device="cuda", generator=G)
+    _, _, lp = R.rows(x, ids, 1.0)
+    old, ref = (lp - 0.05).float(), (lp + 0.3).float()  # ratio 1.05: inside the clip on both sides of every step
+    adv = torch.randn(n, device="cuda", generator=G)
+    kw = dict(ref_logp=ref, kl_coef=0.2)
+    _, _, dx = kernel.policy_loss(x, ids, old, adv, **kw)
+    h = 1e-2
+    for k in range(8):
+        u = torch.randn(n, V, device="cuda", generator=gen(20 + k))
+        u /= u.norm(dim=1, keepdim=True)
+        up = kernel.policy_loss(x + h * u, ids, old, adv, **kw, grad=False)[0].double()
+        dn = kernel.policy_loss(x - h * u, ids, old, adv, **kw, grad=False)[0].double()
+        num, ana = (up - dn) / (2 * h), (dx.double() * u.double()).sum(1)
+        size = adv.double().abs() * 1.05 + 0.2 * 2
+        assert bool(((num - ana).abs() <= size * (2e-4 + 2 * 1.3e-5 / h)).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [5, 1000, 40000])
+def test_rows_at_the_edges(V, dtype):
+    """Nothing left of a row; a mask of the type's lowest value; a row of that
+    value alone (uniform); huge values; a masked id; NaN and +inf."""
+    from mstar_rs_b200 import _native as N
+    from mstar_rs_b200 import kernel
+
+    low = torch.finfo(dtype).min
+    x = torch.randn(9, V, device="cuda", generator=gen(V)).to(dtype)
+    ids = torch.full((9,), 2, device="cuda")
+    x[0] = -math.inf                       # empty
+    x[1] = low                             # uniform at the lowest value
+    x[2, 3:] = low                         # masked by it
+    x[3, 1:] = -math.inf                   # one id left, and it is not the sampled one
+    x[4, 2] = 3e38                         # all the weight on the id
+    x[5, 4] = 3e38                         # none of it
+    x[6, 0] = math.nan
+    x[7, 0] = math.inf
+    adv = torch.ones(9, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    logp, lse = kernel.token_logprobs(x, ids, status=status)
+    assert status.item() == N.STATUS_EMPTY
+    _, rl, rp = R.rows(x[:6], ids[:6], 1.0)
+    assert logp[0] == -math.inf and lse[0] == -math.inf and logp[3] == -math.inf
+    for i in (1, 2, 4, 5):
+        assert abs(logp[i].double() - rp[i]) <= R.SUM + rp[i].abs() * 2.0 ** -23, i
+    assert bool(torch.isnan(logp[6:8]).all()) and bool(torch.isfinite(logp[8]))
+    for old in (None, torch.zeros(9, device="cuda")):
+        loss, lp, dx = kernel.policy_loss(x, ids, old, adv, clip_high=1e30)
+        assert torch.equal(lp.nan_to_num(1.0), logp.nan_to_num(1.0))
+        assert loss[0] == 0 and bool((dx[0] == 0).all())           # empty: no loss, no gradient
+        assert bool((dx[3] == 0).all())                            # a masked id: no gradient
+        assert bool(torch.isfinite(loss[1:6]).all()) and bool(torch.isfinite(dx[:6].float()).all())
+        assert bool(torch.isnan(loss[6:8]).all())
+        r = torch.ones(()) if old is None else logp[1].exp().cpu()  # the uniform row: -r (onehot - 1/V)
+        want = torch.full((V,), float(r) / V, dtype=torch.float64)
+        want[2] -= float(r)
+        near(dx[1].cpu(), want, want.abs() * (R.HALF[dtype] + 2e-5) + float(r) * 2.0 ** -22)
+        assert bool((dx[2, 3:] == 0).all())
+    g = kernel.token_logprobs_grad(x, ids, lse, adv)
+    assert bool((g[0] == 0).all()) and bool((g[2, 3:] == 0).all()) and bool(torch.isfinite(g[8].float()).all())
+
+
+def test_rows_strided_and_misaligned():
+    """Rows inside a wider matrix, starting at an odd column, gradients into
+    another layout: only the rows' own columns are written."""
+    from mstar_rs_b200 import kernel
+
+    n, V = 6, 999
+    for dtype in (BF16, F32):
+        for off in (1, 3, 5):
+            wide = torch.randn(n, V + 31, device="cuda", generator=gen(off)).to(dtype)
+            x = wide[:, off:off + V]
+            ids = torch.randint(0, V, (n,), device="cuda", generator=gen(2))
+            to = torch.full((n, V + 12), 5.0, device="cuda").to(dtype)
+            adv = torch.randn(n, device="cuda", generator=gen(3))
+            _, _, dx = kernel.policy_loss(x, ids, None, adv)
+            _, _, dy = kernel.policy_loss(x, ids, None, adv, dlogits=to[:, 2:2 + V])
+            assert torch.equal(dx, dy) and bool((to[:, :2] == 5).all()) and bool((to[:, 2 + V:] == 5).all())
+            logp, lse = kernel.token_logprobs(x, ids)
+            want = kernel.token_logprobs_grad(x.contiguous(), ids, lse, adv)
+            got = kernel.token_logprobs_grad(x, ids, lse, adv, out=to[:, 1:1 + V])
+            assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------ together, streams, graphs
+
+
+def test_a_rollout_and_its_update():
+    """The operators as they are used together: look up the sampled ids in
+    the tied 4-bit table, project with it, sample, take the log-probabilities
+    of what was sampled, then the policy loss on the same logits and the
+    gradient of the lookup; captured once and replayed, each step equal to
+    the eager calls'."""
+    from mstar_rs_b200 import _native as N
+    from mstar_rs_b200 import kernel
+
+    B, V, d = 12, 5003, 256
+    w = torch.randn(V, d, device="cuda", generator=gen(1)) * 0.2
+    codes, scales, zeros = kernel.quantize_w4(w, 64, zero_points=True)
+    seed = torch.arange(B, dtype=torch.int64, device="cuda")
+
+    def step(ids, offset, logits):
+        x = kernel.embed_tokens_w4(ids, codes, scales, zeros=zeros, scale=math.sqrt(d))
+        out = torch.empty_like(ids)
+        kernel.lmhead_step_w4(x, codes, scales, logits, zeros=zeros, seed=seed, offset=offset, out_ids=out,
+                              flags=N.FLAG_ADVANCE_OFFSET)
+        logp, lse = kernel.token_logprobs(logits, out)
+        loss, lp, dl = kernel.policy_loss(logits, out, logp, torch.ones_like(logp))
+        dx = (dl @ w).to(BF16)
+        dw = kernel.embed_tokens_grad(ids, dx, V, scale=math.sqrt(d), dtype=F32)
+        return out, logp, loss, lp, dl, dw
+
+    ids0 = torch.randint(0, V, (B,), device="cuda", generator=gen(2))
+    off_e = torch.zeros(B, dtype=torch.int64, device="cuda")
+    eager, ids = [], ids0
+    for _ in range(3):
+        r = step(ids, off_e, torch.empty(B, V, device="cuda"))
+        eager.append([t.clone() for t in r])
+        ids = r[0]
+    assert bool((eager[0][1] == eager[0][3]).all())  # both take the same log-probabilities
+    near(eager[0][2], torch.full((B,), -1.0, dtype=torch.float64, device="cuda"), 1e-6)  # ratio 1, advantage 1
+
+    gids, goff, glog = ids0.clone(), torch.zeros_like(off_e), torch.empty(B, V, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = step(gids, goff, glog)
+    for want in eager:
+        g.replay()
+        for a, b in zip(res, want):
+            assert torch.equal(a, b)
+        gids.copy_(res[0])
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, and two captured graphs replayed on two streams:
+    each has its own scratch."""
+    from mstar_rs_b200 import kernel
+
+    V, d = 20000, 512
+    codes, scales, _ = w4_inputs(V, d, 128, BF16, False, 5)
+    hs = [torch.randn(b, d, device="cuda", generator=gen(b)).to(BF16) for b in (3, 40)]
+    ids = [torch.randint(0, 900, (n,), device="cuda", generator=gen(n)) for n in (5000, 7000)]
+    douts = [torch.randn(len(i), 96, device="cuda", generator=gen(9)).to(BF16) for i in ids]
+    one = lambda k: (kernel.lmhead_logits_w4(hs[k], codes, scales), kernel.embed_tokens_grad(ids[k], douts[k], 900))  # noqa: E731
+    want = [one(k) for k in (0, 1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(one(k))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(torch.equal(a, b) for r in got[k] for a, b in zip(r, want[k]))
+    graphs = []
+    for k in (0, 1):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            r = one(k)
+        graphs.append((g, r))
+    for _ in range(5):
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(torch.equal(a, b) for a, b in zip(graphs[k][1], want[k]))
