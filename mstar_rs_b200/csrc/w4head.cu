@@ -12,14 +12,24 @@
 // to it turning the codes into bf16 (some 1.4 instructions per weight), so the
 // kernel overlaps the two: one persistent CTA per SM takes an equal share of
 // the (tile of 256 ids, 256 columns) units.
-//   warps 0-15  workers: a thread owns one vocabulary row and half of each
-//               block of 128 columns: codes from shared memory to bf16 pairs
-//               in registers to tensor memory (the A operand; no second trip
-//               through shared memory), and for half of the batch the group
-//               sums back from tensor memory into its fp32 accumulators;
+//   warps 0-7   expanders: a thread owns one vocabulary row: codes from shared
+//               memory to bf16 pairs in registers to tensor memory (the A
+//               operand; no second trip through shared memory);
+//   warps 8-15  accumulators: a thread owns one vocabulary row and all of the
+//               chunk's batch rows: group sums from tensor memory, times the
+//               group's scale, into fp32 registers;
 //   warp 16     weight producer: TMA boxes of 256 rows x 128 bytes;
 //   warp 17     hidden producer: TMA boxes of 64 columns of the batch;
-//   warp 18     MMA issuer (A from tensor memory, B from shared memory).
+//   warps 18-19 MMA issuers, one per half of the tile (A from tensor memory, B
+//               from shared memory).  With few batch rows an MMA is short and
+//               what bounds the stream is the issuing warp's own chain of
+//               waits and instructions, so the two halves have one each, the
+//               warp stays converged (its operands are then uniform), and
+//               with groups of 128 one barrier says that A is written and
+//               the accumulator free, and one that both are done with.
+// The accumulators hold up to 128 sums per thread, so the warpgroups' shares
+// of the registers are set unequal (setmaxnreg).
+//
 // A word holds eight codes; taking codes i and i + 4 as a pair is one mask
 // and one or per pair, so the pairs' order is [0 4 1 5 2 6 3 7] and a small
 // kernel before puts the hidden columns into it.
@@ -46,8 +56,15 @@ constexpr int BM = 256;            // vocabulary ids per tile: two MMA tiles of 
 constexpr int KS = 256;            // columns per weight stage (128 bytes of codes: one swizzle row)
 constexpr int KB = 128;            // columns per block: one A operand, one hidden stage
 constexpr int W_BYTES = BM * KS / 2;
-constexpr int WORKERS = 512;
-constexpr int THREADS = WORKERS + 96;
+constexpr int ROWS_NT = 256;       // threads of each of the two row roles: one per row of the tile
+constexpr int THREADS = 2 * ROWS_NT + 128;
+// Registers per thread after the split of the 640 * 96 = 61440 that the block
+// is launched with: 128 * (2 * expand + 2 * sum + issue) stays below it.
+template <int N>
+struct Regs {
+  static constexpr int EXPAND = N > 64 ? 56 : 80, SUM = N > 64 ? 160 : 112, ISSUE = N > 64 ? 40 : 56;
+  static_assert(128 * (2 * EXPAND + 2 * SUM + ISSUE) <= THREADS * 96, "registers of the launch");
+};
 constexpr int MAX_WS = 6, MAX_HS = 4;
 constexpr int MAX_N = 128;         // batch rows per chunk
 constexpr int MAX_B = 256;
@@ -95,7 +112,11 @@ struct Work {
 
 struct Sh {
   uint64_t wfull[MAX_WS], wempty[MAX_WS], hfull[MAX_HS], hempty[MAX_HS];
-  uint64_t afull[2][2], aempty[2][2], dfull[2][4], dempty[2][4], mma_done;
+  // Per half of the tile.  Groups of 128 (one per block): ready[j] = A buffer
+  // j written and the block's accumulator free, done[j] = its MMAs complete.
+  // Smaller groups: ready[j] is A's alone and done[j] frees it, dfull and
+  // dempty hand the accumulators over.
+  uint64_t ready[2][2], done[2][2], dfull[2][2], dempty[2][2], mma_done[2];
   uint32_t tmem_base;
   int abort;
   int last;
@@ -107,24 +128,68 @@ __device__ __forceinline__ void raise(const Gemm &g, Sh &sh) {
   if (g.err) atomicOr(g.err, ERR_TIMEOUT);
 }
 
-// Barrier over the worker warps, and-reducing `v`.
-__device__ __forceinline__ int workers_all(int v) {
+// A place in a ring of `n` stages and the parity of its current use.
+struct Ring {
+  uint32_t i = 0, parity = 0;
+  __device__ __forceinline__ void next(uint32_t n) {
+    if (++i == n) i = 0, parity ^= 1u;
+  }
+};
+
+// Warp-wide wait: one look, and the bounded wait behind it.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (__all_sync(~0u, ok)) return true;
+  return __all_sync(~0u, mbar_wait(bar, parity));
+}
+__device__ __forceinline__ void warp_arrive(uint64_t *bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// Barrier over the accumulator warps, and-reducing `v`.
+__device__ __forceinline__ int sums_all(int v) {
   int r;
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n bar.red.and.pred q, 1, 512, p;\n selp.s32 %0, 1, 0, q;\n}\n"
+      "{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n bar.red.and.pred q, 1, 256, p;\n selp.s32 %0, 1, 0, q;\n}\n"
       : "=r"(r)
       : "r"(v)
       : "memory");
   return r;
 }
 
-__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate) {
+// KN / 16 MMAs along the columns of one group: A advances by eight columns of
+// tensor memory, B by 32 bytes of its rows, four steps to a box.  Issued by
+// the lane with `lead` set; the warp is converged.
+template <int KN>
+__device__ __forceinline__ void mma_group(uint32_t lead, uint32_t d, uint32_t a, uint32_t desc_lo, uint32_t desc_hi,
+                                          uint32_t box16, uint32_t idesc) {
+#pragma unroll
+  for (int k = 0; k < KN / 16; ++k)
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .b64 bd;\n setp.ne.b32 q, %0, 0;\n setp.ne.b32 p, %6, 0;\n"
+        " mov.b64 bd, {%3, %4};\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], bd, %5, {%7, %7, %7, %7}, p;\n}\n" ::"r"(lead),
+        "r"(d), "r"(a + 8u * k), "r"(desc_lo + (uint32_t)(k >> 2) * box16 + 2u * (k & 3)), "r"(desc_hi), "r"(idesc),
+        "r"(k ? 1u : 0u), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t lead, uint64_t *bar) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "{\n .reg .pred q;\n setp.ne.b32 q, %0, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n}\n" ::"r"(lead),
+      "r"(smem_u32(bar))
       : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r;
 }
 
 // 16 columns of this warp's 32 lanes, from registers.
@@ -137,11 +202,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
-}
 
 // Eight codes of a word as four bf16 pairs (i, i + 4), each code less the
 // zero point: 0x4300 | q is 128 + q in bf16, and zz holds 128 + z twice.
@@ -179,272 +239,293 @@ __global__ void __launch_bounds__(256)
                      x[3] | (uint32_t)x[7] << 16);
 }
 
+// Waits until each of the ring's last `n` uses (at most its stages) has landed.
+__device__ void drain(const Gemm &g, Sh &sh, uint64_t *full, Ring r, uint32_t n, uint32_t stages) {
+  for (uint32_t j = 0; j < n; ++j) {
+    if (r.i == 0) r.i = stages, r.parity ^= 1u;
+    --r.i;
+    if (!mbar_wait(&full[r.i], r.parity)) raise(g, sh);
+  }
+}
+
 __device__ void produce_weights(const Gemm &g, Sh &sh, uint8_t *sW, const CUtensorMap *map) {
+  // one chunk: every weight is read once; several: their CTAs meet in L2
   const uint64_t pol = g.nchunks == 1 ? policy_evict_first() : policy_evict_last();
-  uint32_t it = 0;
+  const uint32_t stages = (uint32_t)g.wstages;
+  Ring r;
+  uint32_t used = 0;  // stages filled so far, up to the ring's length
   Work w(g);
   bool go = true;
   while (go && w.next(g)) {
-    for (int k = w.k0; k < w.k1 && go; ++k, ++it) {
-      const uint32_t s = it % (uint32_t)g.wstages, use = it / (uint32_t)g.wstages;
-      if (aborted(sh) || (use > 0 && !mbar_wait(&sh.wempty[s], (use - 1) & 1u))) {
+    const int y = w.tile / g.nchunks * BM;
+    for (int k = w.k0; k < w.k1; ++k) {
+      if (aborted(sh) || (used == stages && !mbar_wait(&sh.wempty[r.i], r.parity ^ 1u))) {
         go = false;
         break;
       }
-      mbar_expect_tx(&sh.wfull[s], (uint32_t)W_BYTES);
-      tma_load_2d(sW + (size_t)s * W_BYTES, map, k * (KS / 2), w.tile / g.nchunks * BM, &sh.wfull[s], pol);
+      mbar_expect_tx(&sh.wfull[r.i], (uint32_t)W_BYTES);
+      tma_load_2d(sW + r.i * (uint32_t)W_BYTES, map, k * (KS / 2), y, &sh.wfull[r.i], pol);
+      r.next(stages);
+      used = min(used + 1, stages);
     }
   }
   if (!go) raise(g, sh);
-  for (uint32_t j = it > (uint32_t)g.wstages ? it - (uint32_t)g.wstages : 0; j < it; ++j)  // every copy lands
-    if (!mbar_wait(&sh.wfull[j % (uint32_t)g.wstages], (j / (uint32_t)g.wstages) & 1u)) raise(g, sh);
+  drain(g, sh, sh.wfull, r, used, stages);
 }
 
 __device__ void produce_hidden(const Gemm &g, Sh &sh, uint8_t *sH, const CUtensorMap *map) {
   const uint64_t pol = policy_evict_last();
-  const uint32_t box = (uint32_t)g.n * 128u;
-  uint32_t it = 0;
+  const uint32_t stages = (uint32_t)g.hstages, box = (uint32_t)g.n * 128u;
+  Ring r;
+  uint32_t used = 0;
   Work w(g);
   bool go = true;
   while (go && w.next(g)) {
-    for (int b = w.b0(); b < w.b1(g) && go; ++b, ++it) {
-      const uint32_t s = it % (uint32_t)g.hstages, use = it / (uint32_t)g.hstages;
-      if (aborted(sh) || (use > 0 && !mbar_wait(&sh.hempty[s], (use - 1) & 1u))) {
+    const int y = w.tile % g.nchunks * g.rows, b1 = w.b1(g);
+    for (int b = w.b0(); b < b1; ++b) {
+      if (aborted(sh) || (used == stages && !mbar_wait(&sh.hempty[r.i], r.parity ^ 1u))) {
         go = false;
         break;
       }
-      mbar_expect_tx(&sh.hfull[s], 2u * box);
-      for (int j = 0; j < 2; ++j)
-        tma_load_2d(sH + (size_t)s * 2 * box + (size_t)j * box, map, b * KB + j * 64, w.tile % g.nchunks * g.rows,
-                    &sh.hfull[s], pol);
+      mbar_expect_tx(&sh.hfull[r.i], 2u * box);
+      uint8_t *to = sH + r.i * 2u * box;
+      tma_load_2d(to, map, b * KB, y, &sh.hfull[r.i], pol);
+      tma_load_2d(to + box, map, b * KB + 64, y, &sh.hfull[r.i], pol);
+      r.next(stages);
+      used = min(used + 1, stages);
     }
   }
   if (!go) raise(g, sh);
-  for (uint32_t j = it > (uint32_t)g.hstages ? it - (uint32_t)g.hstages : 0; j < it; ++j)
-    if (!mbar_wait(&sh.hfull[j % (uint32_t)g.hstages], (j / (uint32_t)g.hstages) & 1u)) raise(g, sh);
+  drain(g, sh, sh.hfull, r, used, stages);
 }
 
-template <int NH, int GPB>
-struct Ring {  // accumulators of one tile, one per group in flight
-  static constexpr int N = 2 * NH;
-  static constexpr int ND = N >= 128 ? 1 : N >= 64 ? 2 : 4;
-};
+// Accumulators per half of the tile in tensor memory: one group's sums each.
+template <int N>
+__host__ __device__ constexpr int slots() {
+  return N >= 128 ? 1 : 2;
+}
 
-template <int NH, int GPB>
-__device__ void issue(const Gemm &g, Sh &sh, uint8_t *sH, uint32_t tbase) {
-  constexpr int ND = Ring<NH, GPB>::ND;
-  const uint32_t idesc = idesc_bf16(128, g.n), box = (uint32_t)g.n * 128u, h0 = smem_u32(sH);
-  uint32_t ib = 0, ig = 0;
+template <int N, int GPB>
+__device__ void issue(const Gemm &g, Sh &sh, uint8_t *sH, uint32_t tbase, uint32_t t) {
+  constexpr int ND = slots<N>();
+  const uint32_t lead = elect_one();
+  const uint32_t idesc = idesc_bf16(128, g.n), box16 = (uint32_t)g.n * 8u;
+  const uint64_t h0 = sw128_desc(smem_u32(sH));  // (stages and columns are added in its units of 16 bytes)
+  const uint32_t hlo = (uint32_t)h0, hhi = (uint32_t)(h0 >> 32);
+  const uint32_t hstages = (uint32_t)g.hstages, a0 = tbase + A_COL + t * 128u, d0 = tbase + D_COL + t * 128u;
+  Ring h, a, dd;  // hidden stages, A buffers, accumulators
+  bool first_lap = true, ok = true;
   Work w(g);
-  bool go = true;
-  while (go && w.next(g)) {
-    for (int b = w.b0(); b < w.b1(g) && go; ++b, ++ib) {
-      const uint32_t hs = ib % (uint32_t)g.hstages, buf = ib & 1u;
-      const int groups = min(GPB, (g.d - b * KB) / (KB / GPB));
-      if (aborted(sh) || !mbar_wait(&sh.hfull[hs], (ib / (uint32_t)g.hstages) & 1u)) {
-        go = false;
-        break;
-      }
-      for (uint32_t t = 0; t < 2 && go; ++t) {
-        if (!mbar_wait(&sh.afull[t][buf], (ib >> 1) & 1u)) {
-          go = false;
-          break;
-        }
-        for (int gi = 0; gi < groups; ++gi) {
-          const uint32_t q = ig + (uint32_t)gi, j = q % ND, use = q / ND;
-          if (use > 0 && !mbar_wait(&sh.dempty[t][j], (use - 1) & 1u)) {
-            go = false;
-            break;
-          }
+  while (ok && w.next(g)) {
+    const int b1 = w.b1(g);
+    for (int b = w.b0(); b < b1; ++b) {
+      ok = warp_wait(&sh.hfull[h.i], h.parity) && warp_wait(&sh.ready[t][a.i], a.parity);
+      if (!ok) break;
+      const uint32_t lo = hlo + h.i * 2u * box16;
+      if (GPB == 1) {
+        tc_fence_after();
+        mma_group<KB>(lead, d0 + (ND == 2 ? a.i : 0u) * (uint32_t)N, a0 + a.i * 64u, lo, hhi, box16, idesc);
+      } else {
+        const int groups = min(GPB, (g.d - b * KB) / (KB / GPB));
+#pragma unroll
+        for (int gi = 0; gi < GPB; ++gi) {
+          if (gi >= groups) break;
+          if (!first_lap && !(ok = warp_wait(&sh.dempty[t][dd.i], dd.parity ^ 1u))) break;
           tc_fence_after();
-          const uint32_t dcol = tbase + D_COL + t * 128u + j * (uint32_t)(2 * NH);
-#pragma unroll
-          for (int k = 0; k < KB / GPB / 16; ++k) {
-            const uint32_t kk = (uint32_t)(gi * (KB / GPB / 16) + k);  // sixteen columns each
-            mma_ts(dcol, tbase + A_COL + t * 128u + buf * 64u + kk * 8u,
-                   sw128_desc(h0 + hs * 2u * box + (kk >> 2) * box + (kk & 3u) * 32u), idesc, k ? 1u : 0u);
-          }
-          mma_commit(&sh.dfull[t][j]);
+          constexpr int KN = KB / GPB;
+          mma_group<KN>(lead, d0 + dd.i * (uint32_t)N, a0 + a.i * 64u + gi * (KN / 2),
+                        lo + (uint32_t)(gi * KN / 64) * box16 + (uint32_t)(gi * KN % 64) / 8u, hhi, box16, idesc);
+          commit(lead, &sh.dfull[t][dd.i]);
+          dd.next(ND);
+          if (dd.i == 0) first_lap = false;
         }
-        mma_commit(&sh.aempty[t][buf]);
+        if (!ok) break;
       }
-      ig += (uint32_t)groups;
-      mma_commit(&sh.hempty[hs]);
+      commit(lead, &sh.done[t][a.i]);
+      commit(lead, &sh.hempty[h.i]);
+      h.next(hstages);
+      a.next(2);
     }
   }
-  if (!go) raise(g, sh);
-  mma_commit(&sh.mma_done);  // every MMA issued is complete before tensor memory is released
-  if (!mbar_wait(&sh.mma_done, 0)) raise(g, sh);
+  if (!ok) raise(g, sh);
+  commit(lead, &sh.mma_done[t]);  // every MMA issued is complete before tensor memory is released
+  if (!warp_wait(&sh.mma_done[t], 0)) raise(g, sh);
 }
 
-template <int NH, int GPB>
-struct Worker {
-  static constexpr int ND = Ring<NH, GPB>::ND;
-  static constexpr int LC = NH >= 64 ? 16 : NH;  // columns per load: the accumulators leave no room for more
-  const Gemm &g;
-  Sh &sh;
-  uint8_t *sW;
-  uint32_t tbase;
-  int lane, quad, t, h, row;
-  bool ok = true;
-  float acc[NH];
-  uint32_t ib = 0, ig = 0, is = 0;  // blocks, groups and stages so far
-
-  __device__ Worker(const Gemm &g_, Sh &sh_, uint8_t *sW_, uint32_t tb) : g(g_), sh(sh_), sW(sW_), tbase(tb) {
-    const int warp = threadIdx.x >> 5;
-    lane = threadIdx.x & 31;
-    quad = warp & 3;  // tensor memory lanes 32 * quad .. + 31 belong to this warp
-    t = (warp >> 2) & 1;
-    h = warp >> 3;
-    row = t * 128 + quad * 32 + lane;
-  }
-  __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity) {
-    if (ok && !__all_sync(~0u, mbar_wait(bar, parity))) {
-      ok = false;
-      raise(g, sh);
-    }
-  }
-  __device__ __forceinline__ void arrive(uint64_t *bar) {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar);
-  }
-  __device__ __forceinline__ float scale_at(int v, int G) const {
-    if (v >= g.V || G >= g.ngroups) return 0.f;
-    const int64_t at = (int64_t)v * g.ngroups + G;
-    return g.scale_dtype == MSTAR_DTYPE_F32 ? __ldg(static_cast<const float *>(g.scales) + at)
-                                            : __bfloat162float(static_cast<const __nv_bfloat16 *>(g.scales)[at]);
-  }
-  __device__ __forceinline__ uint32_t zero_at(int v, int G) const {
-    if (!g.zeros || v >= g.V || G >= g.ngroups) return 8u;
-    return __ldg(g.zeros + (int64_t)v * g.ngroups + G) & 15u;
-  }
-  // the group sums of one block into the accumulators
-  __device__ __forceinline__ void drain(int b, const float (&s)[GPB]) {
-    const int groups = min(GPB, (g.d - b * KB) / (KB / GPB));
+// Codes to bf16 in tensor memory, one vocabulary row per thread.
+template <int GPB>
+__device__ void expand_rows(const Gemm &g, Sh &sh, const uint8_t *sW, uint32_t tbase) {
+  const int warp = (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int t = warp >> 2, quad = warp & 3, row = t * 128 + quad * 32 + lane;
+  const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + A_COL + (uint32_t)t * 128u;
+  const uint8_t *mine = sW + (size_t)row * (KS / 2);
+  const uint32_t swz = (uint32_t)(row & 7);
+  Ring st, a;
+  bool first_lap = true;
+  Work w(g);
+  while (w.next(g)) {
+    const int b0 = w.b0(), b1 = w.b1(g);
+    const uint8_t *zp = nullptr;
+    if (g.zeros) zp = g.zeros + (int64_t)min(w.tile / g.nchunks * BM + row, g.V - 1) * g.ngroups;
+    uint32_t z[GPB], zn[GPB];
 #pragma unroll
-    for (int gi = 0; gi < GPB; ++gi) {
-      if (gi >= groups) break;
-      const uint32_t j = ig % ND;
-      wait(&sh.dfull[t][j], (ig / ND) & 1u);
-      ++ig;
-      if (!ok) return;
+    for (int i = 0; i < GPB; ++i) z[i] = zn[i] = 8u;
+    auto fetch = [&](int b) {  // (clamped: groups past the end are never used)
+#pragma unroll
+      for (int i = 0; i < GPB; ++i) zn[i] = __ldg(zp + min(b * GPB + i, g.ngroups - 1));
+    };
+    if (zp) fetch(b0);
+    for (int b = b0; b < b1; ++b) {
+      if (zp) {
+#pragma unroll
+        for (int i = 0; i < GPB; ++i) z[i] = zn[i] & 15u;
+        fetch(b + 1);
+      }
+      if (!(b & 1) && !warp_wait(&sh.wfull[st.i], st.parity)) return raise(g, sh);
+      uint4 c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // 32 columns: 16 bytes of codes
+        c[i] = *reinterpret_cast<const uint4 *>(mine + st.i * (uint32_t)W_BYTES +
+                                                (((uint32_t)((b & 1) * 4 + i) ^ swz) << 4));
+      if (!first_lap && !warp_wait(&sh.done[t][a.i], a.parity ^ 1u)) return raise(g, sh);
       tc_fence_after();
-      const uint32_t at = tbase + ((uint32_t)(quad * 32) << 16) + D_COL + (uint32_t)t * 128u +
-                          j * (uint32_t)(2 * NH) + (uint32_t)(h * NH);
+      const uint32_t at = at0 + a.i * 64u;
 #pragma unroll
-      for (int c0 = 0; c0 < NH; c0 += LC) {
-        uint32_t r[LC];
-#pragma unroll
-        for (int c = 0; c < LC; c += 8) tmem_ld8(at + (uint32_t)(c0 + c), r + c);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < LC; ++c) acc[c0 + c] = fmaf(s[gi], __uint_as_float(r[c]), acc[c0 + c]);
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat16 zf = __ushort_as_bfloat16((unsigned short)(0x4300u | z[i * GPB / 4]));
+        const __nv_bfloat162 zz = __halves2bfloat162(zf, zf);
+        uint32_t r[16];
+        expand(c[i].x, zz, r);
+        expand(c[i].y, zz, r + 4);
+        expand(c[i].z, zz, r + 8);
+        expand(c[i].w, zz, r + 12);
+        tmem_st16(at + (uint32_t)i * 16u, r);
       }
+      if ((b & 1) || b + 1 == b1) {  // (the codes are in registers)
+        warp_arrive(&sh.wempty[st.i]);
+        st.next((uint32_t)g.wstages);
+      }
+      tmem_wait_st();
       tc_fence_before();
-      arrive(&sh.dempty[t][j]);
+      warp_arrive(&sh.ready[t][a.i]);
+      a.next(2);
+      if (a.i == 0) first_lap = false;
     }
   }
-  __device__ __forceinline__ void put(int v, int chunk) {
-    const uint64_t pol = policy_evict_last();
-    if (v >= g.V) return;
+}
+
+template <int N>
+__device__ __forceinline__ void put(const Gemm &g, int v, int chunk, const float (&acc)[N]) {
+  if (v >= g.V) return;
+  const uint64_t pol = policy_evict_last();
+  const int b0 = chunk * g.rows, n = min(g.rows, g.B - b0);
+  if (g.out_dtype == MSTAR_DTYPE_BF16) {
+    __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(g.out) + (int64_t)b0 * g.ld + v;
 #pragma unroll
-    for (int c = 0; c < NH; ++c) {
-      const int col = h * NH + c, b = chunk * g.rows + col;
-      if (col < g.rows && b < g.B) {
-        if (g.out_dtype == MSTAR_DTYPE_BF16)
-          st_last(static_cast<__nv_bfloat16 *>(g.out) + (int64_t)b * g.ld + v, __float2bfloat16_rn(acc[c]), pol);
-        else
-          st_last(static_cast<float *>(g.out) + (int64_t)b * g.ld + v, acc[c], pol);
-      }
-    }
+    for (int c = 0; c < N; ++c, p += g.ld)
+      if (c < n) st_last(p, __float2bfloat16_rn(acc[c]), pol);
+  } else {
+    float *p = static_cast<float *>(g.out) + (int64_t)b0 * g.ld + v;
+#pragma unroll
+    for (int c = 0; c < N; ++c, p += g.ld)
+      if (c < n) st_last(p, acc[c], pol);
   }
-  __device__ __forceinline__ bool segment(const Work &w) {
+}
+
+// Group sums times scales, one vocabulary row per thread.
+template <int N, int GPB>
+__device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
+  const int warp = (int)(threadIdx.x >> 5) - 8, lane = threadIdx.x & 31;
+  const int t = warp >> 2, quad = warp & 3, row = t * 128 + quad * 32 + lane;
+  const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + D_COL + (uint32_t)t * 128u;
+  const bool f32 = g.scale_dtype == MSTAR_DTYPE_F32;
+  constexpr int ND = slots<N>();
+  Ring dd;  // groups of 128: the done barriers, otherwise the accumulators
+  if (GPB == 1)
+    for (int j = 0; j < ND; ++j) warp_arrive(&sh.ready[t][j]);  // the first blocks' accumulators are free
+  Work w(g);
+  while (w.next(g)) {
     const int v = w.tile / g.nchunks * BM + row, chunk = w.tile % g.nchunks;
     const int b0 = w.b0(), b1 = w.b1(g);
-    float s[GPB], sn[GPB];
-    uint32_t z[2], zn[2];  // this half's groups: one, or two of 32 columns
+    const int64_t s0 = (int64_t)min(v, g.V - 1) * g.ngroups;
+    float acc[N], s[GPB], sn[GPB];
 #pragma unroll
-    for (int c = 0; c < NH; ++c) acc[c] = 0.f;
+    for (int c = 0; c < N; ++c) acc[c] = 0.f;
     auto fetch = [&](int b) {
 #pragma unroll
-      for (int gi = 0; gi < GPB; ++gi) sn[gi] = scale_at(v, b * GPB + gi);
-      zn[0] = zero_at(v, b * GPB + h * GPB / 2);
-      zn[1] = GPB == 4 ? zero_at(v, b * GPB + h * GPB / 2 + 1) : zn[0];
+      for (int i = 0; i < GPB; ++i) {
+        const int64_t at = s0 + min(b * GPB + i, g.ngroups - 1);
+        sn[i] = f32 ? __ldg(static_cast<const float *>(g.scales) + at)
+                    : __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(g.scales) + at));
+      }
     };
     fetch(b0);
-    for (int b = b0; b < b1; ++b, ++ib) {
-      const uint32_t st = is % (uint32_t)g.wstages, buf = ib & 1u;
-      float sp[GPB];  // the previous block's scales: its sums are drained after this block's codes are out
+    bool ok = true;
+    for (int b = b0; b < b1 && ok; ++b) {
 #pragma unroll
-      for (int gi = 0; gi < GPB; ++gi) sp[gi] = s[gi], s[gi] = sn[gi];
-      z[0] = zn[0], z[1] = zn[1];
-      if (b + 1 < b1) fetch(b + 1);
-      if (!(b & 1)) wait(&sh.wfull[st], (is / (uint32_t)g.wstages) & 1u);
-      if (ib >= 2) wait(&sh.aempty[t][buf], ((ib >> 1) - 1) & 1u);
-      if (ok) {
-        tc_fence_after();
-        const uint8_t *base = sW + (size_t)st * W_BYTES + (size_t)row * (KS / 2);
-        const uint32_t at = tbase + ((uint32_t)(quad * 32) << 16) + A_COL + (uint32_t)t * 128u + buf * 64u +
-                            (uint32_t)h * 32u;
+      for (int i = 0; i < GPB; ++i) s[i] = sn[i];
+      fetch(b + 1);
+      const int groups = min(GPB, (g.d - b * KB) / (KB / GPB));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {  // 32 columns: 16 bytes of codes
-          const uint32_t piece = (uint32_t)((b & 1) * 4 + h * 2 + i) ^ (uint32_t)(row & 7);
-          const uint4 c = *reinterpret_cast<const uint4 *>(base + piece * 16u);
-          const __nv_bfloat16 zf = __ushort_as_bfloat16((unsigned short)(0x4300u | z[i]));
-          const __nv_bfloat162 zz = __halves2bfloat162(zf, zf);
-          uint32_t r[16];
-          expand(c.x, zz, r);
-          expand(c.y, zz, r + 4);
-          expand(c.z, zz, r + 8);
-          expand(c.w, zz, r + 12);
-          tmem_st16(at + (uint32_t)i * 16u, r);
+      for (int gi = 0; gi < GPB; ++gi) {
+        if (gi >= groups) break;
+        if (!warp_wait(GPB == 1 ? &sh.done[t][dd.i] : &sh.dfull[t][dd.i], dd.parity)) {
+          ok = false;
+          break;
         }
-        tmem_wait_st();
+        tc_fence_after();
+        const uint32_t at = at0 + (ND == 1 ? 0u : dd.i * (uint32_t)N);
+#pragma unroll
+        for (int c0 = 0; c0 < N; c0 += 16) {
+          uint32_t r[16];
+          tmem_ld16(at + (uint32_t)c0, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 16; ++c) acc[c0 + c] = fmaf(s[gi], __uint_as_float(r[c]), acc[c0 + c]);
+        }
         tc_fence_before();
-        arrive(&sh.afull[t][buf]);
-        if ((b & 1) || b + 1 == b1) arrive(&sh.wempty[st]);
+        // (with one accumulator it is the next block's, with two the next but one's)
+        warp_arrive(GPB > 1 ? &sh.dempty[t][dd.i] : &sh.ready[t][ND == 1 ? dd.i ^ 1u : dd.i]);
+        dd.next(GPB == 1 ? 2 : ND);
       }
-      if ((b & 1) || b + 1 == b1) ++is;
-      if (b > b0) drain(b - 1, sp);
     }
-    drain(b1 - 1, s);
-    if (!workers_all(ok)) return false;
+    if (!ok) raise(g, sh);
+    if (!sums_all(ok)) return;
     if (w.k0 == 0 && w.k1 == g.nks) {
-      put(v, chunk);
-      return true;
+      put<N>(g, v, chunk, acc);
+      continue;
     }
     // a shared tile: leave the part, and let the last to come add them all
     const int n = g.n;
-    float *mine = g.parts + ((size_t)blockIdx.x * 2 + (w.k0 == 0 ? 1 : 0)) * (size_t)n * BM;
+    float *part = g.parts + ((size_t)blockIdx.x * 2 + (w.k0 == 0 ? 1 : 0)) * (size_t)n * BM + row;
 #pragma unroll
-    for (int c = 0; c < NH; ++c)
-      if (h * NH + c < n) __stcg(mine + (size_t)(h * NH + c) * BM + row, acc[c]);
+    for (int c = 0; c < N; ++c)
+      if (c < n) __stcg(part + c * BM, acc[c]);
     __threadfence();
-    workers_all(1);
+    sums_all(1);
     const uint32_t first = (uint32_t)w.tile * (uint32_t)g.nks, end = first + (uint32_t)g.nks;
     int c_lo = blockIdx.x, c_hi = blockIdx.x + 1;
     while (c_lo > 0 && unit_start(g, c_lo) > first) --c_lo;
     while (c_hi < (int)gridDim.x && unit_start(g, c_hi) < end) ++c_hi;
-    if (threadIdx.x == 0) sh.last = (int)atomicAdd(&g.counters[w.tile], 1u) == c_hi - c_lo - 1;
-    workers_all(1);
+    if (threadIdx.x == ROWS_NT) sh.last = (int)atomicAdd(&g.counters[w.tile], 1u) == c_hi - c_lo - 1;
+    sums_all(1);
     const bool last = *reinterpret_cast<volatile int *>(&sh.last) != 0;
-    workers_all(1);  // everyone has read it
-    if (!last) return true;
+    sums_all(1);  // everyone has read it
+    if (!last) continue;
     __threadfence();
 #pragma unroll
-    for (int c = 0; c < NH; ++c) acc[c] = 0.f;
+    for (int c = 0; c < N; ++c) acc[c] = 0.f;
     for (int q = c_lo; q < c_hi; ++q) {
       const float *p = g.parts + ((size_t)q * 2 + (unit_start(g, q) <= first ? 1 : 0)) * (size_t)n * BM + row;
 #pragma unroll
-      for (int c = 0; c < NH; ++c)
-        if (h * NH + c < n) acc[c] += __ldcg(p + (size_t)(h * NH + c) * BM);
+      for (int c = 0; c < N; ++c)
+        if (c < n) acc[c] += __ldcg(p + c * BM);
     }
-    put(v, chunk);
-    return true;
+    put<N>(g, v, chunk, acc);
   }
-};
+}
 
-template <int NH, int GPB>
+template <int N, int GPB>
 __global__ void __launch_bounds__(THREADS, 1)
     w4_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap th, const Gemm g) {
   extern __shared__ __align__(1024) uint8_t w4_smem_raw[];
@@ -456,23 +537,23 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < MAX_WS; ++s) {
       mbar_init(&sh.wfull[s], 1);
-      mbar_init(&sh.wempty[s], WORKERS / 32);
+      mbar_init(&sh.wempty[s], ROWS_NT / 32);
     }
     for (int s = 0; s < MAX_HS; ++s) {
       mbar_init(&sh.hfull[s], 1);
-      mbar_init(&sh.hempty[s], 1);
+      mbar_init(&sh.hempty[s], 2);
     }
     for (int t = 0; t < 2; ++t) {
       for (int j = 0; j < 2; ++j) {
-        mbar_init(&sh.afull[t][j], WORKERS / 64);
-        mbar_init(&sh.aempty[t][j], 1);
+        mbar_init(&sh.ready[t][j], GPB == 1 ? 2 * ROWS_NT / 64 : ROWS_NT / 64);
+        mbar_init(&sh.done[t][j], 1);
       }
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2; ++j) {
         mbar_init(&sh.dfull[t][j], 1);
-        mbar_init(&sh.dempty[t][j], WORKERS / 64);
+        mbar_init(&sh.dempty[t][j], ROWS_NT / 64);
       }
+      mbar_init(&sh.mma_done[t], 1);
     }
-    mbar_init(&sh.mma_done, 1);
     sh.abort = 0;
     fence_barrier_init();
   }
@@ -487,19 +568,24 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tbase = sh.tmem_base;
   // the weights do not come from the kernel before; the hidden rows and the
   // counters do, and the output may still be read by what ran before that
-  if (warp != 16) asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (warp == 16) {
-    if (lane == 0) produce_weights(g, sh, sW, &tw);
-  } else if (warp == 17) {
-    asm volatile("fence.proxy.async;" ::: "memory");
-    if (lane == 0) produce_hidden(g, sh, sH, &th);
-  } else if (warp == 18) {
-    if (lane == 0) issue<NH, GPB>(g, sh, sH, tbase);
+  if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<N>::EXPAND));
+    expand_rows<GPB>(g, sh, sW, tbase);
+  } else if (warp < 16) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<N>::SUM));
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    sum_rows<N, GPB>(g, sh, tbase);
   } else {
-    Worker<NH, GPB> me(g, sh, sW, tbase);
-    Work w(g);
-    while (w.next(g))
-      if (!me.segment(w)) break;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<N>::ISSUE));
+    if (warp == 16) {
+      if (lane == 0) produce_weights(g, sh, sW, &tw);
+    } else if (warp == 17) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      asm volatile("fence.proxy.async;" ::: "memory");
+      if (lane == 0) produce_hidden(g, sh, sH, &th);
+    } else {
+      issue<N, GPB>(g, sh, sH, tbase, (uint32_t)warp - 18u);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -559,9 +645,9 @@ static int make_map(CUtensorMap *m, CUtensorMapDataType type, int size, const vo
   return MSTAR_OK;
 }
 
-template <int NH, int GPB>
+template <int N, int GPB>
 static int launch(const CUtensorMap &tw, const CUtensorMap &th, const Gemm &g, cudaStream_t st) {
-  auto kern = w4_gemm_kernel<NH, GPB>;
+  auto kern = w4_gemm_kernel<N, GPB>;
   const int smem = g.wstages * W_BYTES + g.hstages * g.n * KB * 2 + 1024;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
@@ -580,11 +666,11 @@ static int launch(const CUtensorMap &tw, const CUtensorMap &th, const Gemm &g, c
   return MSTAR_OK;
 }
 
-template <int NH>
+template <int N>
 static int launch_n(const CUtensorMap &tw, const CUtensorMap &th, const Gemm &g, cudaStream_t st) {
-  return g.group == 128 ? launch<NH, 1>(tw, th, g, st)
-         : g.group == 64 ? launch<NH, 2>(tw, th, g, st)
-                         : launch<NH, 4>(tw, th, g, st);
+  return g.group == 128 ? launch<N, 1>(tw, th, g, st)
+         : g.group == 64 ? launch<N, 2>(tw, th, g, st)
+                         : launch<N, 4>(tw, th, g, st);
 }
 
 static int logits(const void *hidden, int64_t ldh, int B, const mstar_w4_t *w, void *out, int dtype, int64_t ld,
@@ -624,10 +710,10 @@ static int logits(const void *hidden, int64_t ldh, int B, const mstar_w4_t *w, v
                                                                 g.ntt);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e));
-  if (g.n <= 16) return launch_n<8>(tw, th, g, st);
-  if (g.n <= 32) return launch_n<16>(tw, th, g, st);
-  if (g.n <= 64) return launch_n<32>(tw, th, g, st);
-  return launch_n<64>(tw, th, g, st);
+  if (g.n <= 16) return launch_n<16>(tw, th, g, st);
+  if (g.n <= 32) return launch_n<32>(tw, th, g, st);
+  if (g.n <= 64) return launch_n<64>(tw, th, g, st);
+  return launch_n<128>(tw, th, g, st);
 }
 
 }  // namespace w4
