@@ -4,44 +4,55 @@
 //   logits[b, v] = sum_G s[v, G] * sum_{k in G} hidden[b, k] * (q[v, k] - z[v, G])
 //
 // A code less its zero point is a whole number of at most four bits and a
-// sign, exact in bf16; so is every product with a bf16 hidden value in the
-// tensor core's fp32 accumulator.  The scale is applied to each group's sum,
-// in fp32: rounding q * s to bf16 instead would cost 2^-9 of every weight.
+// sign, exact in fp16; so is every product with a hidden value in the tensor
+// core's fp32 accumulator.  The scale is applied to each group's sum, in fp32:
+// rounding q * s to 16 bits instead would cost 2^-9 or 2^-12 of every weight.
+// The operands are fp16 and not bf16 because its ten bits take a code at two
+// places of a word (below), which spares two of seven integer instructions;
+// so each hidden row is first scaled by a power of two that brings its largest
+// value into [2^14, 2^15).  A bf16 value keeps all its bits down to 2^-31 of the
+// row's largest and is off by at most 2^-40 of that below.
 //
 // With few rows the weight stream bounds the product (V * d / 2 bytes), next
-// to it turning the codes into bf16 (some 1.4 instructions per weight), so the
-// kernel overlaps the two: one persistent CTA per SM takes an equal share of
-// the (tile of 256 ids, 256 columns) units.
-//   warps 0-7   expanders: a thread owns one vocabulary row: codes from shared
-//               memory to bf16 pairs in registers to tensor memory (the A
-//               operand; no second trip through shared memory);
-//   warps 8-15  accumulators: a thread owns one vocabulary row and all of the
-//               chunk's batch rows: group sums from tensor memory, times the
-//               group's scale, into fp32 registers;
-//   warp 16     weight producer: TMA boxes of 256 rows x 128 bytes;
-//   warp 17     hidden producer: TMA boxes of 64 columns of the batch;
-//   warps 18-19 MMA issuers, one per half of the tile (A from tensor memory, B
-//               from shared memory).  With few batch rows an MMA is short and
-//               what bounds the stream is the issuing warp's own chain of
-//               waits and instructions, so the two halves have one each, the
-//               warp stays converged (its operands are then uniform), and
-//               with groups of 128 one barrier says that A is written and
-//               the accumulator free, and one that both are done with.
-// The accumulators hold up to 128 sums per thread, so the warpgroups' shares
-// of the registers are set unequal (setmaxnreg).
+// to it turning the codes into fp16 (nine instructions for eight weights) and
+// storing them to tensor memory, so the kernel overlaps the three: one
+// persistent CTA per SM takes an equal share of the (tile of 256 ids, 256
+// columns) units.
+//   expanders    a thread owns a vocabulary row: codes from shared memory to
+//                fp16 pairs in registers to tensor memory (the A operand; no
+//                second trip through shared memory);
+//   accumulators a thread owns a vocabulary row and the chunk's batch rows:
+//                group sums from tensor memory, times the group's scale, into
+//                fp32 registers;
+//   producers    a warp for the weights (TMA boxes of 256 rows x 128 bytes)
+//                and one for the hidden rows (boxes of 64 columns);
+//   MMA issuers  converged warps (their operands are then uniform);
+//   counter      a warp that counts the parts of tiles shared between CTAs.
+// What bounds such a pipeline are its hand-overs: a wait, a few dependent
+// instructions and an arrival cost each role some hundred cycles, next to the
+// 735 in which memory delivers a block of 256 x 128 codes.  So the two blocks
+// of a stage have an A buffer, accumulators, expander warps and issuers of
+// their own (up to 64 batch rows), each of which has twice the time; with
+// groups of 128 one barrier says that A is written and the accumulator free,
+// and one that both are done with.
 //
-// A word holds eight codes; taking codes i and i + 4 as a pair is one mask
-// and one or per pair, so the pairs' order is [0 4 1 5 2 6 3 7] and a small
+// A word holds eight codes; codes i and i + 4 are a pair: one instruction masks
+// them and sets fp16's exponent (0x6400 | q is 1024 + q; at bits 4-7 it is
+// 1024 + 16 q), one subtracts.  The pairs' order is [0 4 1 5 2 6 3 7] and the
 // kernel before puts the hidden columns into it.
 //
-// A tile that several CTAs share is summed by whichever of them comes last,
-// in the order of the columns: nobody waits for anybody, and the sum does
-// not depend on who was last.
+// A tile that several CTAs share is summed by the one whose part comes last, in
+// the order of the columns: no CTA waits for another, and the sum does not
+// depend on which it is.  A CTA takes its shared tiles first and adds at its
+// end, so that neither the count nor the parts are waited for (counting and
+// adding at once held the accumulators up by 8 of 51 us; B=1, V=151936,
+// d=2048).
 //
 // Every wait is bounded; one that runs out sets the error word, the roles
 // stop issuing, drain what they issued, and the CTA exits.
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -56,27 +67,48 @@ constexpr int BM = 256;            // vocabulary ids per tile: two MMA tiles of 
 constexpr int KS = 256;            // columns per weight stage (128 bytes of codes: one swizzle row)
 constexpr int KB = 128;            // columns per block: one A operand, one hidden stage
 constexpr int W_BYTES = BM * KS / 2;
-constexpr int ROWS_NT = 256;       // threads of each of the two row roles: one per row of the tile
-constexpr int THREADS = 2 * ROWS_NT + 128;
-// Registers per thread after the split of the 640 * 96 = 61440 that the block
-// is launched with: 128 * (2 * expand + 2 * sum + issue) stays below it.
+// Roles by the accumulator's width N.  LANES: whether the two blocks of a
+// stage have expanders and issuers of their own.  The registers per thread
+// that each role keeps of those that the block is launched with are set by
+// setmaxnreg.
 template <int N>
-struct Regs {
-  static constexpr int EXPAND = N > 64 ? 56 : 80, SUM = N > 64 ? 160 : 112, ISSUE = N > 64 ? 40 : 56;
-  static_assert(128 * (2 * EXPAND + 2 * SUM + ISSUE) <= THREADS * 96, "registers of the launch");
+struct Roles {
+  static constexpr int LANES = N > 32 ? 1 : 2;
+  static constexpr int EXPAND = 8 * LANES;                       // expander warps: 32 rows of the tile each
+  static constexpr int SUM = 8;                                  // accumulator warps: the same
+  static constexpr int ISSUE = 2 * LANES;                        // a warp per half of the tile
+  static constexpr int REST = 8;  // 2 producers, the issuers, the counting warp, in whole warpgroups
+  static constexpr int THREADS = 32 * (EXPAND + SUM + REST);
+  static constexpr int LAUNCH = 65536 / THREADS / 8 * 8;
+  static constexpr int REGS_EXPAND = N > 64 ? 48 : N > 32 ? 72 : 64;
+  static constexpr int REGS_SUM = N > 64 ? 160 : N > 32 ? 120 : 80;
+  static constexpr int REGS_REST = N > 64 ? 32 : 48;
+  static_assert(32 * (EXPAND * REGS_EXPAND + SUM * REGS_SUM + REST * REGS_REST) <= THREADS * LAUNCH,
+                "registers of the launch");
+  // Tensor memory: A buffers [2 blocks][2 tiles][64 columns], then the
+  // accumulators [slot][2 tiles][N].  A block's groups take its lane's slots in
+  // turn; with one lane the blocks share the slots.
+  static constexpr int D_COL = 256;
+  static constexpr int SLOTS = N > 64 ? 1 : N > 32 ? 2 : 4;
+  static constexpr int RING = SLOTS / LANES;  // slots per lane
+  // One barrier for A written and the accumulator free, one for both done.
+  template <int GPB>
+  static __host__ __device__ constexpr bool merged() {
+    return GPB == 1 && RING == 1;
+  }
 };
-constexpr int MAX_WS = 6, MAX_HS = 4;
+constexpr int MAX_WS = 6, MAX_HS = 8;
 constexpr int MAX_N = 128;         // batch rows per chunk
 constexpr int MAX_B = 256;
 constexpr int SMEM_BUDGET = 220 * 1024;
 constexpr uint32_t ERR_TIMEOUT = 1u;
-constexpr uint32_t A_COL = 0, D_COL = 256;  // tensor memory: [tile][buffer] of A, then the accumulators
 
 struct Gemm {
   int B, V, d;
   int rows, nchunks, n;   // batch rows per chunk, chunks, MMA N (rows rounded up to 16)
   int nks, nblk, ntt;     // stages and blocks along d; tiles times chunks
   int wstages, hstages;
+  uint32_t share, longer; // units per CTA, and how many CTAs take one more
   int group, ngroups;
   const void *scales;
   int scale_dtype;
@@ -85,47 +117,96 @@ struct Gemm {
   int64_t ld;
   int out_dtype;
   uint32_t *err;
+  const float *row_scale; // [B] what the hidden rows were divided by
   uint32_t *counters;     // [ntt] parts of a shared tile that have arrived
   float *parts;           // [grid][2][n][BM]
 };
 
+// Shares are equal to within one unit: CTA c's begins at c * share + min(c, longer).
 __device__ __forceinline__ uint32_t unit_start(const Gemm &g, int c) {
-  return (uint32_t)((uint64_t)g.ntt * (uint64_t)g.nks * (uint64_t)c / gridDim.x);
+  return (uint32_t)c * g.share + min((uint32_t)c, g.longer);
 }
 
-// This CTA's share as segments: stages [k0, k1) of one tile.
+// This CTA's share as segments, stages [k0, k1) of one tile: the tile it shares
+// with the next CTA, the one it shares with the one before, then whole tiles.
 struct Work {
-  uint32_t u, u1;
   int tile, k0, k1;
-  __device__ explicit Work(const Gemm &g) : u(unit_start(g, blockIdx.x)), u1(unit_start(g, blockIdx.x + 1)) {}
+  int t0, r0, t1, r1, at;
+  __device__ explicit Work(const Gemm &g) : at(0) {
+    const uint32_t u0 = unit_start(g, blockIdx.x), u1 = unit_start(g, blockIdx.x + 1);
+    t0 = (int)(u0 / (uint32_t)g.nks), r0 = (int)(u0 % (uint32_t)g.nks);
+    t1 = (int)(u1 / (uint32_t)g.nks), r1 = (int)(u1 % (uint32_t)g.nks);
+  }
   __device__ bool next(const Gemm &g) {
-    if (u >= u1) return false;
-    tile = (int)(u / (uint32_t)g.nks);
-    k0 = (int)(u % (uint32_t)g.nks);
-    k1 = min(g.nks, k0 + (int)(u1 - u));
-    u += (uint32_t)(k1 - k0);
-    return true;
+    if (at == 0) {
+      ++at;
+      if (r1 > 0) {
+        tile = t1, k0 = t0 == t1 ? r0 : 0, k1 = r1;
+        return true;
+      }
+    }
+    if (at == 1) {
+      ++at;
+      tile = t0 - 1;
+      if (r0 > 0) {
+        tile = t0, k0 = r0, k1 = g.nks;
+        if (t0 < t1) return true;
+      }
+    }
+    k0 = 0, k1 = g.nks;
+    if (at == 2) ++at, tile = r0 > 0 ? t0 : t0 - 1;
+    return ++tile < t1;
   }
   __device__ int b0() const { return 2 * k0; }
   __device__ int b1(const Gemm &g) const { return min(2 * k1, g.nblk); }
 };
 
+// The CTAs [c_lo, c_hi) whose shares meet `tile`.
+__device__ __forceinline__ void sharers(const Gemm &g, int tile, int &c_lo, int &c_hi) {
+  const uint32_t first = (uint32_t)tile * (uint32_t)g.nks, end = first + (uint32_t)g.nks;
+  c_lo = blockIdx.x, c_hi = blockIdx.x + 1;
+  while (c_lo > 0 && unit_start(g, c_lo) > first) --c_lo;
+  while (c_hi < (int)gridDim.x && unit_start(g, c_hi) < end) ++c_hi;
+}
+
 struct Sh {
   uint64_t wfull[MAX_WS], wempty[MAX_WS], hfull[MAX_HS], hempty[MAX_HS];
-  // Per half of the tile.  Groups of 128 (one per block): ready[j] = A buffer
-  // j written and the block's accumulator free, done[j] = its MMAs complete.
-  // Smaller groups: ready[j] is A's alone and done[j] frees it, dfull and
-  // dempty hand the accumulators over.
-  uint64_t ready[2][2], done[2][2], dfull[2][2], dempty[2][2], mma_done[2];
+  // By half of the tile t and block of the stage j.  Groups of 128 (one per
+  // block): ready[t][j] = A written and the block's accumulator free,
+  // done[t][j] = its MMAs complete.  Smaller groups: ready is A's alone and
+  // done frees it, dfull and dempty [t][slot] hand the accumulators over.
+  uint64_t ready[2][2], done[2][2], dfull[2][4], dempty[2][4], mma_done[4];
   uint32_t tmem_base;
   int abort;
-  int last;
+  int last[2];  // whether this CTA's part of the tile shared with the CTA before / after was the last
 };
 
 __device__ __forceinline__ bool aborted(const Sh &sh) { return *reinterpret_cast<const volatile int *>(&sh.abort); }
 __device__ __forceinline__ void raise(const Gemm &g, Sh &sh) {
   *reinterpret_cast<volatile int *>(&sh.abort) = 1;
   if (g.err) atomicOr(g.err, ERR_TIMEOUT);
+}
+
+// The hot loops name barriers by their shared-memory address and keep what a
+// hand-over costs to a few instructions: a pipeline of waits is bound by them.
+//
+// Waits for phase `parity`, at most LOOKS looks at the barrier (each of which
+// may sleep until the phase ends; some ten milliseconds in all, and no
+// less than one), and sets `late` if they run out.
+constexpr uint32_t LOOKS = 1u << 16;
+__device__ __forceinline__ void await(uint32_t bar, uint32_t parity, uint32_t &late) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
+      "LOOK:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra SEEN;\n"
+      " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra LOOK;\n mov.u32 %0, 1;\nSEEN:\n}\n"
+      : "+r"(late)
+      : "r"(bar), "r"(parity), "n"(LOOKS)
+      : "memory");
+}
+// One arrival of the whole warp.
+__device__ __forceinline__ void arrive(uint32_t bar, bool lane0) {
+  __syncwarp();
+  if (lane0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // A place in a ring of `n` stages and the parity of its current use.
@@ -136,32 +217,11 @@ struct Ring {
   }
 };
 
-// Warp-wide wait: one look, and the bounded wait behind it.
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  if (__all_sync(~0u, ok)) return true;
-  return __all_sync(~0u, mbar_wait(bar, parity));
-}
-__device__ __forceinline__ void warp_arrive(uint64_t *bar) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
-
-// Barrier over the accumulator warps, and-reducing `v`.
-__device__ __forceinline__ int sums_all(int v) {
-  int r;
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n bar.red.and.pred q, 1, 256, p;\n selp.s32 %0, 1, 0, q;\n}\n"
-      : "=r"(r)
-      : "r"(v)
-      : "memory");
-  return r;
-}
+// Named barriers 1 and 2 tell the counting warp that a part of this CTA's two
+// shared tiles is written (the accumulator warps arrive and go on); barrier 3
+// tells them what it counted.
+__device__ __forceinline__ void bar_arrive(int id) { asm volatile("bar.arrive %0, 288;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void bar_sync(int id) { asm volatile("bar.sync %0, 288;" ::"r"(id) : "memory"); }
 
 // KN / 16 MMAs along the columns of one group: A advances by eight columns of
 // tensor memory, B by 32 bytes of its rows, four steps to a box.  Issued by
@@ -179,11 +239,11 @@ __device__ __forceinline__ void mma_group(uint32_t lead, uint32_t d, uint32_t a,
         "r"(k ? 1u : 0u), "r"(0u)
         : "memory");
 }
-__device__ __forceinline__ void commit(uint32_t lead, uint64_t *bar) {
+__device__ __forceinline__ void commit(uint32_t lead, uint32_t bar) {
   asm volatile(
       "{\n .reg .pred q;\n setp.ne.b32 q, %0, 0;\n"
       " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n}\n" ::"r"(lead),
-      "r"(smem_u32(bar))
+      "r"(bar)
       : "memory");
 }
 __device__ __forceinline__ uint32_t elect_one() {
@@ -203,40 +263,84 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Eight codes of a word as four bf16 pairs (i, i + 4), each code less the
-// zero point: 0x4300 | q is 128 + q in bf16, and zz holds 128 + z twice.
-__device__ __forceinline__ void expand(uint32_t w, __nv_bfloat162 zz, uint32_t *r) {
+// Eight codes of a word as four fp16 pairs (i, i + 4), each code less the
+// zero point: nz holds -(1024 + z) twice, nz16 -(64 + z).
+__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t mask) {
+  uint32_t t;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(t) : "r"(w), "r"(mask), "r"(0x64006400u));
+  return t;
+}
+__device__ __forceinline__ void expand(uint32_t w, uint32_t nz, uint32_t nz16, uint32_t *r) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t t = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-    const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&t), zz);
-    r[i] = *reinterpret_cast<const uint32_t *>(&x);
+  for (int i = 0; i < 4; i += 2) {
+    const uint32_t x = w >> (4 * i);
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(mask_or(x, 0x000F000Fu)), "r"(nz));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[i + 1]) : "r"(mask_or(x, 0x00F000F0u)), "r"(0x2C002C00u), "r"(nz16));
   }
 }
 
-// The hidden rows with each eight columns in the order [0 4 1 5 2 6 3 7], and
-// the arrival counters cleared.
-__global__ void __launch_bounds__(256)
-    w4_prepare_kernel(const __nv_bfloat16 *hidden, int64_t ld, int B, int d, int vec, uint4 *to, uint32_t *counters,
-                      int ncounters) {
+// One CTA per batch row: the hidden row times a power of two, as fp16, each
+// eight columns in the order [0 4 1 5 2 6 3 7]; the power's inverse; and the
+// arrival counters cleared.
+constexpr int PREP_NT = 256;
+__global__ void __launch_bounds__(PREP_NT)
+    w4_prepare_kernel(const __nv_bfloat16 *hidden, int64_t ld, int d, int vec, uint4 *to, float *row_scale,
+                      uint32_t *counters, int ncounters) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int i = (int)(blockIdx.x * 256 + threadIdx.x);
-  for (int j = i; j < ncounters; j += (int)gridDim.x * 256) counters[j] = 0u;
-  const int per = d / 8;
-  if (i >= B * per) return;
-  const int b = i / per, k = (i - b * per) * 8;
-  const __nv_bfloat16 *p = hidden + (int64_t)b * ld + k;
-  uint16_t x[8];
-  if (vec) {
-    const uint4 w = *reinterpret_cast<const uint4 *>(p);
-    x[0] = (uint16_t)w.x, x[1] = (uint16_t)(w.x >> 16), x[2] = (uint16_t)w.y, x[3] = (uint16_t)(w.y >> 16);
-    x[4] = (uint16_t)w.z, x[5] = (uint16_t)(w.z >> 16), x[6] = (uint16_t)w.w, x[7] = (uint16_t)(w.w >> 16);
-  } else {
+  __shared__ uint32_t warp_max[PREP_NT / 32];
+  const int tid = threadIdx.x, per = d / 8;
+  for (int j = (int)blockIdx.x * PREP_NT + tid; j < ncounters; j += (int)gridDim.x * PREP_NT) counters[j] = 0u;
+  const __nv_bfloat16 *row = hidden + (int64_t)blockIdx.x * ld;
+  auto load = [&](int i, uint16_t(&x)[8]) {
+    const __nv_bfloat16 *p = row + i * 8;
+    if (vec) {
+      const uint4 w = *reinterpret_cast<const uint4 *>(p);
+      x[0] = (uint16_t)w.x, x[1] = (uint16_t)(w.x >> 16), x[2] = (uint16_t)w.y, x[3] = (uint16_t)(w.y >> 16);
+      x[4] = (uint16_t)w.z, x[5] = (uint16_t)(w.z >> 16), x[6] = (uint16_t)w.w, x[7] = (uint16_t)(w.w >> 16);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = __bfloat16_as_ushort(p[j]);
+      for (int j = 0; j < 8; ++j) x[j] = __bfloat16_as_ushort(p[j]);
+    }
+  };
+  uint16_t first[8];  // (most rows are one round of the block: they are read once)
+  uint32_t top = 0;
+  for (int i = tid; i < per; i += PREP_NT) {
+    uint16_t x[8];
+    load(i, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (i == tid) first[j] = x[j];
+      const uint32_t mag = x[j] & 0x7FFFu;
+      if (mag < 0x7F80u) top = max(top, mag);  // the largest finite magnitude
+    }
   }
-  to[i] = make_uint4(x[0] | (uint32_t)x[4] << 16, x[1] | (uint32_t)x[5] << 16, x[2] | (uint32_t)x[6] << 16,
-                     x[3] | (uint32_t)x[7] << 16);
+  top = __reduce_max_sync(~0u, top);
+  if ((tid & 31) == 0) warp_max[tid >> 5] = top;
+  __syncthreads();
+  top = 0;
+  for (int w = 0; w < PREP_NT / 32; ++w) top = max(top, warp_max[w]);
+  int e = 0;
+  if (top) {
+    int x;
+    frexpf(__uint_as_float(top << 16), &x);  // the largest is in [2^(x-1), 2^x)
+    e = 15 - x;
+  }
+  if (tid == 0) row_scale[blockIdx.x] = ldexpf(1.f, -e);
+  for (int i = tid; i < per; i += PREP_NT) {
+    uint16_t x[8];
+    if (i == tid) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = first[j];
+    } else {
+      load(i, x);
+    }
+    uint32_t y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      y[j] = __half_as_ushort(__float2half_rn(ldexpf(__uint_as_float((uint32_t)x[j] << 16), e)));
+    to[(int64_t)blockIdx.x * per + i] =
+        make_uint4(y[0] | y[4] << 16, y[1] | y[5] << 16, y[2] | y[6] << 16, y[3] | y[7] << 16);
+  }
 }
 
 // Waits until each of the ring's last `n` uses (at most its stages) has landed.
@@ -299,245 +403,324 @@ __device__ void produce_hidden(const Gemm &g, Sh &sh, uint8_t *sH, const CUtenso
   drain(g, sh, sh.hfull, r, used, stages);
 }
 
-// Accumulators per half of the tile in tensor memory: one group's sums each.
-template <int N>
-__host__ __device__ constexpr int slots() {
-  return N >= 128 ? 1 : 2;
-}
-
+// MMAs of half t of the tile, of the blocks of `lane` (with one lane: of all).
 template <int N, int GPB>
-__device__ void issue(const Gemm &g, Sh &sh, uint8_t *sH, uint32_t tbase, uint32_t t) {
-  constexpr int ND = slots<N>();
+__device__ void issue(const Gemm &g, Sh &sh, uint8_t *sH, uint32_t tbase, int who) {
+  using R = Roles<N>;
+  constexpr int RING = R::RING;
+  constexpr bool MERGED = R::template merged<GPB>();
+  const int t = who & 1, lane = who >> 1;
   const uint32_t lead = elect_one();
-  const uint32_t idesc = idesc_bf16(128, g.n), box16 = (uint32_t)g.n * 8u;
+  const uint32_t idesc = idesc_f16(128, g.n), box16 = (uint32_t)g.n * 8u;
   const uint64_t h0 = sw128_desc(smem_u32(sH));  // (stages and columns are added in its units of 16 bytes)
-  const uint32_t hlo = (uint32_t)h0, hhi = (uint32_t)(h0 >> 32);
-  const uint32_t hstages = (uint32_t)g.hstages, a0 = tbase + A_COL + t * 128u, d0 = tbase + D_COL + t * 128u;
-  Ring h, a, dd;  // hidden stages, A buffers, accumulators
-  bool first_lap = true, ok = true;
+  const uint32_t hlo = (uint32_t)h0, hhi = (uint32_t)(h0 >> 32), hstages = (uint32_t)g.hstages;
+  const uint32_t a0 = tbase + (uint32_t)t * 64u, d0 = tbase + R::D_COL + (uint32_t)(t * N);
+  const uint32_t hfull = smem_u32(sh.hfull), hempty = smem_u32(sh.hempty);
+  const uint32_t ready = smem_u32(sh.ready[t]), done = smem_u32(sh.done[t]);
+  const uint32_t dfull = smem_u32(sh.dfull[t]), dempty = smem_u32(sh.dempty[t]);
+  Ring h;
+  uint32_t rp = 0, dp = 0, fresh = 0xFu;  // parities of ready[t][j] and dempty[t][slot], a bit each; unused slots
+  int slot = 0;                           // within the lane's ring
+  uint32_t late = 0;
   Work w(g);
-  while (ok && w.next(g)) {
-    const int b1 = w.b1(g);
-    for (int b = w.b0(); b < b1; ++b) {
-      ok = warp_wait(&sh.hfull[h.i], h.parity) && warp_wait(&sh.ready[t][a.i], a.parity);
-      if (!ok) break;
-      const uint32_t lo = hlo + h.i * 2u * box16;
-      if (GPB == 1) {
-        tc_fence_after();
-        mma_group<KB>(lead, d0 + (ND == 2 ? a.i : 0u) * (uint32_t)N, a0 + a.i * 64u, lo, hhi, box16, idesc);
-      } else {
-        const int groups = min(GPB, (g.d - b * KB) / (KB / GPB));
+  while (!late && w.next(g)) {
+    for (int k = w.k0; k < w.k1 && !late; ++k) {
 #pragma unroll
-        for (int gi = 0; gi < GPB; ++gi) {
-          if (gi >= groups) break;
-          if (!first_lap && !(ok = warp_wait(&sh.dempty[t][dd.i], dd.parity ^ 1u))) break;
-          tc_fence_after();
-          constexpr int KN = KB / GPB;
-          mma_group<KN>(lead, d0 + dd.i * (uint32_t)N, a0 + a.i * 64u + gi * (KN / 2),
-                        lo + (uint32_t)(gi * KN / 64) * box16 + (uint32_t)(gi * KN % 64) / 8u, hhi, box16, idesc);
-          commit(lead, &sh.dfull[t][dd.i]);
-          dd.next(ND);
-          if (dd.i == 0) first_lap = false;
+      for (int j = 0; j < 2; ++j) {
+        if (j == 1 && 2 * k + 1 >= g.nblk) break;
+        if (R::LANES == 2 && j != lane) {
+          h.next(hstages);
+          continue;
         }
-        if (!ok) break;
+        await(hfull + 8u * h.i, h.parity, late);
+        await(ready + 8u * j, (rp >> j) & 1u, late);
+        rp ^= 1u << j;
+        const uint32_t lo = hlo + h.i * 2u * box16, aj = a0 + (uint32_t)j * 128u;
+        if (MERGED) {
+          tc_fence_after();
+          mma_group<KB>(lead, d0 + (R::LANES == 2 ? j : 0) * 2u * N, aj, lo, hhi, box16, idesc);
+        } else {
+          const int groups = GPB == 1 ? 1 : min(GPB, (g.d - (2 * k + j) * KB) / (KB / GPB));
+#pragma unroll
+          for (int gi = 0; gi < GPB; ++gi) {
+            if (gi >= groups) break;
+            const uint32_t q = (R::LANES == 2 ? j * RING : 0) + slot;
+            if (!((fresh >> q) & 1u)) await(dempty + 8u * q, ((dp >> q) & 1u) ^ 1u, late);
+            fresh &= ~(1u << q);
+            dp ^= 1u << q;
+            tc_fence_after();
+            constexpr int KN = KB / GPB;
+            mma_group<KN>(lead, d0 + q * 2u * N, aj + gi * (KN / 2),
+                          lo + (uint32_t)(gi * KN / 64) * box16 + (uint32_t)(gi * KN % 64) / 8u, hhi, box16, idesc);
+            commit(lead, dfull + 8u * q);
+            if (RING == 2) slot ^= 1;
+          }
+        }
+        commit(lead, done + 8u * j);
+        commit(lead, hempty + 8u * h.i);
+        h.next(hstages);
       }
-      commit(lead, &sh.done[t][a.i]);
-      commit(lead, &sh.hempty[h.i]);
-      h.next(hstages);
-      a.next(2);
     }
   }
-  if (!ok) raise(g, sh);
-  commit(lead, &sh.mma_done[t]);  // every MMA issued is complete before tensor memory is released
-  if (!warp_wait(&sh.mma_done[t], 0)) raise(g, sh);
+  if (late) raise(g, sh);
+  late = 0;
+  commit(lead, smem_u32(&sh.mma_done[who]));  // every MMA issued is complete before tensor memory is released
+  await(smem_u32(&sh.mma_done[who]), 0, late);
+  if (late) raise(g, sh);
 }
 
-// Codes to bf16 in tensor memory, one vocabulary row per thread.
-template <int GPB>
+// Codes to fp16 in tensor memory.
+template <int N, int GPB>
 __device__ void expand_rows(const Gemm &g, Sh &sh, const uint8_t *sW, uint32_t tbase) {
+  using R = Roles<N>;
   const int warp = (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int t = warp >> 2, quad = warp & 3, row = t * 128 + quad * 32 + lane;
-  const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + A_COL + (uint32_t)t * 128u;
-  const uint8_t *mine = sW + (size_t)row * (KS / 2);
-  const uint32_t swz = (uint32_t)(row & 7);
-  Ring st, a;
-  bool first_lap = true;
+  const bool lane0 = lane == 0;
+  const int t = (warp >> 2) & 1, quad = warp & 3, row = t * 128 + quad * 32 + lane, mine = warp >> 3;
+  const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + (uint32_t)t * 64u;
+  const uint32_t stages = (uint32_t)g.wstages;
+  const uint32_t wfull = smem_u32(sh.wfull), wempty = smem_u32(sh.wempty);
+  const uint32_t ready = smem_u32(sh.ready[t]), done = smem_u32(sh.done[t]);
+  // this row's 16-byte pieces of a stage lie swizzled: piece i of block j at (4 j + i) ^ (row & 7)
+  uint32_t piece[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    piece[i] = smem_u32(sW) + (uint32_t)row * (KS / 2) + (((uint32_t)(4 * mine + i) ^ (uint32_t)(row & 7)) << 4);
+  Ring st;
+  uint32_t dp = 0, fresh = 3u;  // parities of done[t][j], a bit each; unused A buffers
+  uint32_t nz[GPB], nz16[GPB], late = 0;
+#pragma unroll
+  for (int i = 0; i < GPB; ++i) nz[i] = 0xE408E408u, nz16[i] = 0xD480D480u;  // zero point 8
   Work w(g);
   while (w.next(g)) {
-    const int b0 = w.b0(), b1 = w.b1(g);
     const uint8_t *zp = nullptr;
     if (g.zeros) zp = g.zeros + (int64_t)min(w.tile / g.nchunks * BM + row, g.V - 1) * g.ngroups;
-    uint32_t z[GPB], zn[GPB];
+    for (int k = w.k0; k < w.k1; ++k) {
+      const bool two = 2 * k + 1 < g.nblk;  // (d's last stage may hold one block)
+      const uint32_t stage = st.i * (uint32_t)W_BYTES;
+      uint32_t z[GPB];
+      auto fetch = [&](int j) {  // (clamped: groups past the end are never used)
 #pragma unroll
-    for (int i = 0; i < GPB; ++i) z[i] = zn[i] = 8u;
-    auto fetch = [&](int b) {  // (clamped: groups past the end are never used)
+        for (int i = 0; i < GPB; ++i) z[i] = __ldg(zp + min((2 * k + j) * GPB + i, g.ngroups - 1));
+      };
+      if (zp) fetch(R::LANES == 2 ? mine : 0);
+      await(wfull + 8u * st.i, st.parity, late);
 #pragma unroll
-      for (int i = 0; i < GPB; ++i) zn[i] = __ldg(zp + min(b * GPB + i, g.ngroups - 1));
-    };
-    if (zp) fetch(b0);
-    for (int b = b0; b < b1; ++b) {
-      if (zp) {
+      for (int pass = 0; pass < 3 - R::LANES; ++pass) {
+        const int j = R::LANES == 2 ? mine : pass;
+        if (j == 1 && !two) {
+          if (R::LANES == 2) arrive(wempty + 8u * st.i, lane0);
+          break;
+        }
+        uint4 c[4];
 #pragma unroll
-        for (int i = 0; i < GPB; ++i) z[i] = zn[i] & 15u;
-        fetch(b + 1);
+        for (int i = 0; i < 4; ++i) {  // 32 columns: 16 bytes of codes
+          const uint32_t from = (R::LANES == 1 && j == 1 ? piece[i] ^ 64u : piece[i]) + stage;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(c[i].x), "=r"(c[i].y), "=r"(c[i].z), "=r"(c[i].w)
+                       : "r"(from));
+        }
+        if (zp) {
+#pragma unroll
+          for (int i = 0; i < GPB; ++i) {
+            const uint32_t zz = (z[i] & 15u) * 0x10001u;
+            nz[i] = 0xE400E400u | zz, nz16[i] = 0xD400D400u | zz << 4;
+          }
+        }
+        if (!((fresh >> j) & 1u)) await(done + 8u * j, ((dp >> j) & 1u) ^ 1u, late);
+        fresh &= ~(1u << j);
+        dp ^= 1u << j;
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t r[16];
+          expand(c[i].x, nz[i * GPB / 4], nz16[i * GPB / 4], r);
+          expand(c[i].y, nz[i * GPB / 4], nz16[i * GPB / 4], r + 4);
+          expand(c[i].z, nz[i * GPB / 4], nz16[i * GPB / 4], r + 8);
+          expand(c[i].w, nz[i * GPB / 4], nz16[i * GPB / 4], r + 12);
+          tmem_st16(at0 + (uint32_t)j * 128u + (uint32_t)i * 16u, r);
+        }
+        if (R::LANES == 2 || j == 1 || !two) arrive(wempty + 8u * st.i, lane0);  // (the codes are in registers)
+        if (R::LANES == 1 && j == 0 && two && zp) fetch(1);
+        tmem_wait_st();
+        tc_fence_before();
+        arrive(ready + 8u * j, lane0);
       }
-      if (!(b & 1) && !warp_wait(&sh.wfull[st.i], st.parity)) return raise(g, sh);
-      uint4 c[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)  // 32 columns: 16 bytes of codes
-        c[i] = *reinterpret_cast<const uint4 *>(mine + st.i * (uint32_t)W_BYTES +
-                                                (((uint32_t)((b & 1) * 4 + i) ^ swz) << 4));
-      if (!first_lap && !warp_wait(&sh.done[t][a.i], a.parity ^ 1u)) return raise(g, sh);
-      tc_fence_after();
-      const uint32_t at = at0 + a.i * 64u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat16 zf = __ushort_as_bfloat16((unsigned short)(0x4300u | z[i * GPB / 4]));
-        const __nv_bfloat162 zz = __halves2bfloat162(zf, zf);
-        uint32_t r[16];
-        expand(c[i].x, zz, r);
-        expand(c[i].y, zz, r + 4);
-        expand(c[i].z, zz, r + 8);
-        expand(c[i].w, zz, r + 12);
-        tmem_st16(at + (uint32_t)i * 16u, r);
-      }
-      if ((b & 1) || b + 1 == b1) {  // (the codes are in registers)
-        warp_arrive(&sh.wempty[st.i]);
-        st.next((uint32_t)g.wstages);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      warp_arrive(&sh.ready[t][a.i]);
-      a.next(2);
-      if (a.i == 0) first_lap = false;
+      if (late) return raise(g, sh);
+      st.next(stages);
     }
   }
 }
 
-template <int N>
-__device__ __forceinline__ void put(const Gemm &g, int v, int chunk, const float (&acc)[N]) {
+// Sixteen of a row's sums to the logits, times what the hidden rows were divided by.
+__device__ __forceinline__ void put16(const Gemm &g, int v, int chunk, int c0, const float *x) {
   if (v >= g.V) return;
   const uint64_t pol = policy_evict_last();
-  const int b0 = chunk * g.rows, n = min(g.rows, g.B - b0);
+  const int b0 = chunk * g.rows + c0, n = min(g.rows - c0, g.B - b0);
+  const float *rs = g.row_scale + b0;
   if (g.out_dtype == MSTAR_DTYPE_BF16) {
     __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(g.out) + (int64_t)b0 * g.ld + v;
 #pragma unroll
-    for (int c = 0; c < N; ++c, p += g.ld)
-      if (c < n) st_last(p, __float2bfloat16_rn(acc[c]), pol);
+    for (int c = 0; c < 16; ++c, p += g.ld)
+      if (c < n) st_last(p, __float2bfloat16_rn(x[c] * rs[c]), pol);
   } else {
     float *p = static_cast<float *>(g.out) + (int64_t)b0 * g.ld + v;
 #pragma unroll
-    for (int c = 0; c < N; ++c, p += g.ld)
-      if (c < n) st_last(p, acc[c], pol);
+    for (int c = 0; c < 16; ++c, p += g.ld)
+      if (c < n) st_last(p, x[c] * rs[c], pol);
   }
 }
 
-// Group sums times scales, one vocabulary row per thread.
+// Two sums at a time: (a0, a1) += (x0, x1) * (s, s).
+__device__ __forceinline__ void fma2(float &a0, float &a1, uint32_t x0, uint32_t x1, float s) {
+  asm("{\n .reg .b64 a, x, s;\n mov.b64 a, {%0, %1};\n mov.b64 x, {%2, %3};\n mov.b64 s, {%4, %4};\n"
+      " fma.rn.f32x2 a, x, s, a;\n mov.b64 {%0, %1}, a;\n}\n"
+      : "+f"(a0), "+f"(a1)
+      : "r"(x0), "r"(x1), "f"(s));
+}
+
+// Group sums times scales.
 template <int N, int GPB>
 __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
-  const int warp = (int)(threadIdx.x >> 5) - 8, lane = threadIdx.x & 31;
+  using R = Roles<N>;
+  constexpr int RING = R::RING;
+  constexpr bool MERGED = R::template merged<GPB>();
+  constexpr int LC = N == 32 ? 32 : 16;  // columns loaded at a time
+  const int warp = (int)(threadIdx.x >> 5) - R::EXPAND, lane = threadIdx.x & 31;
   const int t = warp >> 2, quad = warp & 3, row = t * 128 + quad * 32 + lane;
-  const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + D_COL + (uint32_t)t * 128u;
+  const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + R::D_COL + (uint32_t)(t * N);
   const bool f32 = g.scale_dtype == MSTAR_DTYPE_F32;
-  constexpr int ND = slots<N>();
-  Ring dd;  // groups of 128: the done barriers, otherwise the accumulators
-  if (GPB == 1)
-    for (int j = 0; j < ND; ++j) warp_arrive(&sh.ready[t][j]);  // the first blocks' accumulators are free
+  const bool lane0 = lane == 0;
+  const uint32_t full = smem_u32(MERGED ? sh.done[t] : sh.dfull[t]);
+  const uint32_t ready = smem_u32(sh.ready[t]), dempty = smem_u32(sh.dempty[t]);
+  uint32_t fp = 0, late = 0;  // parities of done[t][j] (groups of 128) or dfull[t][slot], a bit each
+  int slot = 0;
+  if (MERGED)  // the first blocks' accumulators are free
+    for (int j = 0; j < R::LANES; ++j) arrive(ready + 8u * j, lane0);
   Work w(g);
   while (w.next(g)) {
     const int v = w.tile / g.nchunks * BM + row, chunk = w.tile % g.nchunks;
-    const int b0 = w.b0(), b1 = w.b1(g);
     const int64_t s0 = (int64_t)min(v, g.V - 1) * g.ngroups;
-    float acc[N], s[GPB], sn[GPB];
+    float acc[N], s[2][GPB];
 #pragma unroll
     for (int c = 0; c < N; ++c) acc[c] = 0.f;
-    auto fetch = [&](int b) {
+    auto fetch = [&](int j, int b) {  // (clamped: groups past the end are never used)
 #pragma unroll
       for (int i = 0; i < GPB; ++i) {
         const int64_t at = s0 + min(b * GPB + i, g.ngroups - 1);
-        sn[i] = f32 ? __ldg(static_cast<const float *>(g.scales) + at)
-                    : __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(g.scales) + at));
+        s[j][i] = f32 ? __ldg(static_cast<const float *>(g.scales) + at)
+                      : __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(g.scales) + at));
       }
     };
-    fetch(b0);
-    bool ok = true;
-    for (int b = b0; b < b1 && ok; ++b) {
+    fetch(0, w.b0());
+    fetch(1, w.b0() + 1);
+    for (int k = w.k0; k < w.k1 && !late; ++k) {
 #pragma unroll
-      for (int i = 0; i < GPB; ++i) s[i] = sn[i];
-      fetch(b + 1);
-      const int groups = min(GPB, (g.d - b * KB) / (KB / GPB));
+      for (int j = 0; j < 2; ++j) {
+        const int b = 2 * k + j;
+        if (j == 1 && b >= g.nblk) break;
+        const int groups = GPB == 1 ? 1 : min(GPB, (g.d - b * KB) / (KB / GPB));
 #pragma unroll
-      for (int gi = 0; gi < GPB; ++gi) {
-        if (gi >= groups) break;
-        if (!warp_wait(GPB == 1 ? &sh.done[t][dd.i] : &sh.dfull[t][dd.i], dd.parity)) {
-          ok = false;
-          break;
+        for (int gi = 0; gi < GPB; ++gi) {
+          if (gi >= groups) break;
+          const int q = MERGED ? j : (R::LANES == 2 ? j * RING : 0) + (slot >> (R::LANES == 2 ? j : 0) & 1);
+          await(full + 8u * q, (fp >> q) & 1u, late);
+          fp ^= 1u << q;
+          if (RING == 2) slot ^= 1 << (R::LANES == 2 ? j : 0);
+          tc_fence_after();
+          const uint32_t at = at0 + (R::SLOTS == 1 ? 0u : (uint32_t)q * 2u * N);
+#pragma unroll
+          for (int c0 = 0; c0 < N; c0 += LC) {
+            uint32_t r[LC / 16][16];
+#pragma unroll
+            for (int c = 0; c < LC / 16; ++c) tmem_ld16(at + (uint32_t)(c0 + 16 * c), r[c]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < LC; c += 2)
+              fma2(acc[c0 + c], acc[c0 + c + 1], r[c / 16][c % 16], r[c / 16][c % 16 + 1], s[j][gi]);
+          }
+          tc_fence_before();
+          // (with one lane the accumulator is the next block's, otherwise this lane's next)
+          arrive(!MERGED ? dempty + 8u * q : ready + 8u * (R::LANES == 2 ? j : j == 0 && b + 1 < g.nblk ? 1 : 0), lane0);
         }
-        tc_fence_after();
-        const uint32_t at = at0 + (ND == 1 ? 0u : dd.i * (uint32_t)N);
-#pragma unroll
-        for (int c0 = 0; c0 < N; c0 += 16) {
-          uint32_t r[16];
-          tmem_ld16(at + (uint32_t)c0, r);
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < 16; ++c) acc[c0 + c] = fmaf(s[gi], __uint_as_float(r[c]), acc[c0 + c]);
-        }
-        tc_fence_before();
-        // (with one accumulator it is the next block's, with two the next but one's)
-        warp_arrive(GPB > 1 ? &sh.dempty[t][dd.i] : &sh.ready[t][ND == 1 ? dd.i ^ 1u : dd.i]);
-        dd.next(GPB == 1 ? 2 : ND);
+        fetch(j, b + 2);
       }
     }
-    if (!ok) raise(g, sh);
-    if (!sums_all(ok)) return;
+    if (late) raise(g, sh);
     if (w.k0 == 0 && w.k1 == g.nks) {
-      put<N>(g, v, chunk, acc);
+#pragma unroll
+      for (int c0 = 0; c0 < N; c0 += 16)
+        if (!late) put16(g, v, chunk, c0, acc + c0);
       continue;
     }
-    // a shared tile: leave the part, and let the last to come add them all
-    const int n = g.n;
-    float *part = g.parts + ((size_t)blockIdx.x * 2 + (w.k0 == 0 ? 1 : 0)) * (size_t)n * BM + row;
+    // a shared tile: leave the part (the counting warp sees an error by itself)
+    const int which = w.k0 == 0 ? 1 : 0, cols = min(g.rows, g.B - chunk * g.rows);
+    float *part = g.parts + ((size_t)blockIdx.x * 2 + which) * (size_t)g.n * BM + row;
 #pragma unroll
     for (int c = 0; c < N; ++c)
-      if (c < n) __stcg(part + c * BM, acc[c]);
-    __threadfence();
-    sums_all(1);
-    const uint32_t first = (uint32_t)w.tile * (uint32_t)g.nks, end = first + (uint32_t)g.nks;
-    int c_lo = blockIdx.x, c_hi = blockIdx.x + 1;
-    while (c_lo > 0 && unit_start(g, c_lo) > first) --c_lo;
-    while (c_hi < (int)gridDim.x && unit_start(g, c_hi) < end) ++c_hi;
-    if (threadIdx.x == ROWS_NT) sh.last = (int)atomicAdd(&g.counters[w.tile], 1u) == c_hi - c_lo - 1;
-    sums_all(1);
-    const bool last = *reinterpret_cast<volatile int *>(&sh.last) != 0;
-    sums_all(1);  // everyone has read it
-    if (!last) continue;
-    __threadfence();
+      if (c < cols) __stcg(part + c * BM, acc[c]);
+    bar_arrive(1 + which);
+  }
+  // the shared tiles for which this CTA's part was the last: add the parts in the order of the columns
+  bar_sync(3);
+  Work again(g);
+  while (again.next(g)) {
+    const int which = again.k0 == 0 ? 1 : 0;
+    if ((again.k0 == 0 && again.k1 == g.nks) || !sh.last[which]) continue;
+    const int v = again.tile / g.nchunks * BM + row;
+    const uint32_t first = (uint32_t)again.tile * (uint32_t)g.nks;
+    int c_lo, c_hi;
+    sharers(g, again.tile, c_lo, c_hi);
+    const int chunk = again.tile % g.nchunks, cols = min(g.rows, g.B - chunk * g.rows);
+#pragma unroll 1
+    for (int c0 = 0; c0 < cols; c0 += 16) {
+      float sum[16] = {};
+      for (int q = c_lo; q < c_hi; ++q) {
+        const float *p = g.parts + ((size_t)q * 2 + (unit_start(g, q) <= first ? 1 : 0)) * (size_t)g.n * BM + row;
+        float x[16];  // (columns past the last read it again: no load waits for another)
 #pragma unroll
-    for (int c = 0; c < N; ++c) acc[c] = 0.f;
-    for (int q = c_lo; q < c_hi; ++q) {
-      const float *p = g.parts + ((size_t)q * 2 + (unit_start(g, q) <= first ? 1 : 0)) * (size_t)n * BM + row;
+        for (int c = 0; c < 16; ++c) x[c] = __ldcg(p + min(c0 + c, cols - 1) * BM);
 #pragma unroll
-      for (int c = 0; c < N; ++c)
-        if (c < n) acc[c] += __ldcg(p + c * BM);
+        for (int c = 0; c < 16; ++c) sum[c] += x[c];
+      }
+      put16(g, v, chunk, c0, sum);
     }
-    put<N>(g, v, chunk, acc);
   }
 }
 
+// Counts the parts of the shared tiles as they are written.
+__device__ void count_parts(const Gemm &g, Sh &sh, int lane) {
+  Work w(g);
+  while (w.next(g)) {
+    if (w.k0 == 0 && w.k1 == g.nks) continue;
+    const int which = w.k0 == 0 ? 1 : 0;
+    bar_sync(1 + which);
+    if (lane == 0) {
+      int c_lo, c_hi;
+      sharers(g, w.tile, c_lo, c_hi);
+      __threadfence();  // this CTA's part before the count
+      sh.last[which] = !aborted(sh) && (int)atomicAdd(&g.counters[w.tile], 1u) == c_hi - c_lo - 1;
+      __threadfence();  // the count before the others' parts
+    }
+    __syncwarp();
+  }
+  bar_arrive(3);
+}
+
 template <int N, int GPB>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Roles<N>::THREADS, 1)
     w4_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap th, const Gemm g) {
+  using R = Roles<N>;
   extern __shared__ __align__(1024) uint8_t w4_smem_raw[];
   __shared__ Sh sh;
   uint8_t *smem = w4_smem_raw + ((1024u - (smem_u32(w4_smem_raw) & 1023u)) & 1023u);
   uint8_t *sW = smem, *sH = smem + (size_t)g.wstages * W_BYTES;
+  constexpr int FIRST = R::EXPAND + R::SUM;  // the weight producer's warp; the hidden rows' and the issuers' follow
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int s = 0; s < MAX_WS; ++s) {
       mbar_init(&sh.wfull[s], 1);
-      mbar_init(&sh.wempty[s], ROWS_NT / 32);
+      mbar_init(&sh.wempty[s], R::EXPAND);
     }
     for (int s = 0; s < MAX_HS; ++s) {
       mbar_init(&sh.hfull[s], 1);
@@ -545,19 +728,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int t = 0; t < 2; ++t) {
       for (int j = 0; j < 2; ++j) {
-        mbar_init(&sh.ready[t][j], GPB == 1 ? 2 * ROWS_NT / 64 : ROWS_NT / 64);
+        mbar_init(&sh.ready[t][j], 4 + (R::template merged<GPB>() ? 4 : 0));
         mbar_init(&sh.done[t][j], 1);
       }
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 4; ++j) {
         mbar_init(&sh.dfull[t][j], 1);
-        mbar_init(&sh.dempty[t][j], ROWS_NT / 64);
+        mbar_init(&sh.dempty[t][j], 4);
       }
-      mbar_init(&sh.mma_done[t], 1);
     }
+    for (int j = 0; j < 4; ++j) mbar_init(&sh.mma_done[j], 1);
     sh.abort = 0;
     fence_barrier_init();
   }
-  if (warp == 18) {
+  if (warp == FIRST) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem_base))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -568,29 +751,32 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tbase = sh.tmem_base;
   // the weights do not come from the kernel before; the hidden rows and the
   // counters do, and the output may still be read by what ran before that
-  if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<N>::EXPAND));
-    expand_rows<GPB>(g, sh, sW, tbase);
-  } else if (warp < 16) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<N>::SUM));
+  if (warp < R::EXPAND) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::REGS_EXPAND));
+    expand_rows<N, GPB>(g, sh, sW, tbase);
+  } else if (warp < FIRST) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R::REGS_SUM));
     asm volatile("griddepcontrol.wait;" ::: "memory");
     sum_rows<N, GPB>(g, sh, tbase);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<N>::ISSUE));
-    if (warp == 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::REGS_REST));
+    if (warp == FIRST) {
       if (lane == 0) produce_weights(g, sh, sW, &tw);
-    } else if (warp == 17) {
+    } else if (warp == FIRST + 1) {
       asm volatile("griddepcontrol.wait;" ::: "memory");
       asm volatile("fence.proxy.async;" ::: "memory");
       if (lane == 0) produce_hidden(g, sh, sH, &th);
-    } else {
-      issue<N, GPB>(g, sh, sH, tbase, (uint32_t)warp - 18u);
+    } else if (warp < FIRST + 2 + R::ISSUE) {
+      issue<N, GPB>(g, sh, sH, tbase, warp - FIRST - 2);
+    } else if (warp == FIRST + 2 + R::ISSUE) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      count_parts(g, sh, lane);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 18) {
+  if (warp == FIRST) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tbase) : "memory");
   }
@@ -609,18 +795,20 @@ static Gemm plan(int B, int V, int d) {
   g.nks = (d + KS - 1) / KS;
   g.nblk = (d + KB - 1) / KB;
   g.ntt = (V + BM - 1) / BM * g.nchunks;
-  g.hstages = g.n <= 32 ? 4 : 3;
+  // (64 rows, V=151936, d=2048: 83 us with three hidden stages, 77 with four)
+  g.hstages = g.n <= 16 ? 8 : g.n <= 32 ? 6 : g.n <= 64 ? 5 : 3;
   g.wstages = std::min(MAX_WS, (SMEM_BUDGET - g.hstages * g.n * KB * 2) / W_BYTES);
   return g;
 }
 
 static int grid_of(const Gemm &g) { return (int)std::min<int64_t>(sm_count(), (int64_t)g.ntt * g.nks); }
 
-// Workspace: arrival counters, the reordered hidden rows, the parts of shared
-// tiles; each rounded to 256 bytes.
+// Workspace: arrival counters, the hidden rows as operands, their scales, the
+// parts of shared tiles; each rounded to 256 bytes.
 static int64_t up(int64_t b) { return (b + 255) / 256 * 256; }
 static int64_t hidden_at(const Gemm &g) { return up((int64_t)g.ntt * 4); }
-static int64_t parts_at(const Gemm &g) { return hidden_at(g) + up((int64_t)g.B * g.d * 2); }
+static int64_t scale_at(const Gemm &g) { return hidden_at(g) + up((int64_t)g.B * g.d * 2); }
+static int64_t parts_at(const Gemm &g) { return scale_at(g) + up((int64_t)g.B * 4); }
 static int64_t workspace_bytes(const Gemm &g) { return parts_at(g) + (int64_t)grid_of(g) * 2 * g.n * BM * 4; }
 
 static int check_sizes(int B, int V, int d) {
@@ -653,7 +841,7 @@ static int launch(const CUtensorMap &tw, const CUtensorMap &th, const Gemm &g, c
   if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid_of(g), 1, 1);
-  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.blockDim = dim3(Roles<N>::THREADS, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -689,6 +877,9 @@ static int logits(const void *hidden, int64_t ldh, int B, const mstar_w4_t *w, v
   Gemm g = plan(B, w->V, w->d);
   if (ws_bytes < workspace_bytes(g)) return fail(MSTAR_ERR_INVALID, "workspace too small");
   uint8_t *p = static_cast<uint8_t *>(ws);
+  const uint32_t units = (uint32_t)g.ntt * (uint32_t)g.nks, grid = (uint32_t)grid_of(g);
+  g.share = units / grid;
+  g.longer = units % grid;
   g.group = w->group;
   g.ngroups = w->d / w->group;
   g.scales = w->scales;
@@ -703,11 +894,12 @@ static int logits(const void *hidden, int64_t ldh, int B, const mstar_w4_t *w, v
   void *perm = p + hidden_at(g);
   CUtensorMap tw, th;
   if ((rc = make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w->codes, w->V, w->d / 2, KS / 2, BM))) return rc;
-  if ((rc = make_map(&th, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, perm, B, w->d, 64, g.n))) return rc;
+  if ((rc = make_map(&th, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, perm, B, w->d, 64, g.n))) return rc;
   const int vec = (reinterpret_cast<uintptr_t>(hidden) % 16 == 0 && ldh % 8 == 0) ? 1 : 0;
-  w4_prepare_kernel<<<(B * (w->d / 8) + 255) / 256, 256, 0, st>>>(static_cast<const __nv_bfloat16 *>(hidden), ldh, B,
-                                                                w->d, vec, static_cast<uint4 *>(perm), g.counters,
-                                                                g.ntt);
+  float *row_scale = reinterpret_cast<float *>(p + scale_at(g));
+  g.row_scale = row_scale;
+  w4_prepare_kernel<<<B, PREP_NT, 0, st>>>(static_cast<const __nv_bfloat16 *>(hidden), ldh, w->d, vec,
+                                           static_cast<uint4 *>(perm), row_scale, g.counters, g.ntt);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e));
   if (g.n <= 16) return launch_n<16>(tw, th, g, st);
