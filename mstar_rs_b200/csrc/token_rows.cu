@@ -4,13 +4,19 @@
 //   x = logits / T,  lse = log sum_v exp(x_v),  logp = x_id - lse
 //   d logp / d logits_v = (onehot_v - exp(x_v - lse)) / T
 //
-// One thread-block cluster of S CTAs takes a row; each CTA reads its slice
-// once, in 16-byte vectors, keeping per thread a running maximum and a sum
-// of exponentials (one pass, no separate search for the maximum), which the
-// threads, the warps and (over distributed shared memory) the CTAs join.  The
-// policy loss writes the gradient in the same pass: the slice stays in shared
-// memory, each thread re-reading only the vectors that it stored itself, so
-// the logits are read from memory once and the gradient written once.
+// One thread-block cluster of S CTAs takes a row; each CTA passes once over its
+// slice, in 16-byte vectors, keeping per thread a running maximum and a sum
+// of exponentials (no separate search for the maximum), which the threads,
+// the warps and (over distributed shared memory) the CTAs join.  The policy
+// loss writes the gradient in the same launch and reads the slice again for
+// it, from L2: the rows in flight (148 SMs x 6 CTAs x 76 KB of 151936 bf16)
+// fit there, so memory sees each logit once.  Keeping the slice in shared
+// memory instead left room for too few CTAs to cover the joins (577 against
+// 470 us for 4096 such rows).
+//
+// What bounds it: memory (4 bytes per bf16 logit, read and written: 380 us for
+// 4096 x 151936 at 6553 GB/s), and close behind it the special-function unit
+// (two exponentials per logit at 16 a cycle and SM: 328 us).
 //
 // Arithmetic: exponents are kept in units of log 2, t = x * c - M with c =
 // log2(e) / T rounded to 32 bits and M the (scaled, rounded) running maximum.
@@ -36,8 +42,7 @@ namespace rows {
 constexpr int NT = 256;
 constexpr int NW = NT / 32;
 constexpr int MAX_S = 8;                  // portable cluster width
-constexpr int SLICE_BYTES = 48 * 1024;    // four slices share an SM's shared memory
-constexpr int MAX_RESIDENT = 200 * 1024;  // larger slices are read from memory twice
+constexpr int SLICE_BYTES = 80 * 1024;  // of a row per CTA, where there are rows enough
 // Values at or below FLOOR count as masked while the running maximum is
 // tracked (a mask of the type's lowest value would overflow when scaled by
 // c); a row whose largest value is not inside (FLOOR, -FLOOR) takes the
@@ -50,7 +55,6 @@ struct Args {
   const void *logits;
   int64_t ld;
   int32_t N, V, S;
-  int32_t slice_vecs;  // vectors of shared memory per CTA (POLICY_GRAD, resident)
   const int64_t *ids;
   float c;             // log2(e) / T
   double inv_t;
@@ -62,6 +66,7 @@ struct Args {
   uint32_t *status;
 };
 
+// A 16-byte vector as floats, its largest value, and back.
 template <typename T>
 struct Vec;
 template <>
@@ -72,6 +77,9 @@ struct Vec<float> {
     x[1] = __uint_as_float(w.y);
     x[2] = __uint_as_float(w.z);
     x[3] = __uint_as_float(w.w);
+  }
+  static __device__ __forceinline__ float largest(const uint4 &w) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
   }
   static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
@@ -87,6 +95,11 @@ struct Vec<__nv_bfloat16> {
       x[2 * i] = __uint_as_float(u[i] << 16);
       x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
     }
+  }
+  static __device__ __forceinline__ float largest(const uint4 &w) {
+    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&w);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
     uint32_t u[4];
@@ -124,33 +137,58 @@ struct Row {
   __device__ __forceinline__ const uint4 *vecs() const { return reinterpret_cast<const uint4 *>(p + head); }
 };
 
-// Running (maximum, sum) in scaled units: s = sum 2^(x c - M).
-struct Stat {
-  float m, M, s;  // raw maximum, scaled maximum, sum
-  __device__ explicit Stat(float c) : m(FLOOR), M(FLOOR * c), s(0.f) {}
-  template <int E>
-  __device__ __forceinline__ void add(const float (&x)[E], float c) {
-    float mx = x[0];
+// Calls f(i) for i = first, first + NT, ... below `end`, with the vectors of
+// U of them loaded before any is used: f gets the index and the vector.
+template <int U, typename Load, typename F>
+__device__ __forceinline__ void each_vector(int first, int end, Load load, F f) {
+  int v = first;
+  for (; v + (U - 1) * NT < end; v += U * NT) {
+    uint4 w[U];
 #pragma unroll
-    for (int i = 1; i < E; ++i) mx = fmaxf(mx, x[i]);
+    for (int u = 0; u < U; ++u) w[u] = load(v + u * NT);
+#pragma unroll
+    for (int u = 0; u < U; ++u) f(v + u * NT, w[u]);
+  }
+  if (v < end) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (v + u * NT < end) w[u] = load(v + u * NT);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (v + u * NT < end) f(v + u * NT, w[u]);
+  }
+}
+
+// Running (maximum, sum) in scaled units: s = sum 2^(x c - M), in two halves.
+struct Stat {
+  float m, M, s0, s1;  // raw maximum, scaled maximum, sums
+  __device__ explicit Stat(float c) : m(FLOOR), M(FLOOR * c), s0(0.f), s1(0.f) {}
+  __device__ __forceinline__ void raise(float mx, float c) {
     if (mx > m) {
-      const float M2 = mx * c;
-      s *= ex2(M - M2);
+      const float M2 = mx * c, f = ex2(M - M2);
+      s0 *= f;
+      s1 *= f;
       m = mx;
       M = M2;
     }
-    float part = 0.f;
+  }
+  template <typename T>
+  __device__ __forceinline__ void add(const uint4 &w, float c) {
+    raise(Vec<T>::largest(w), c);
+    float x[Vec<T>::E];
+    Vec<T>::unpack(w, x);
 #pragma unroll
-    for (int i = 0; i < E; ++i) part += ex2(fmaf(x[i], c, -M));
-    s += part;
+    for (int i = 0; i < Vec<T>::E; i += 2) {
+      s0 += ex2(fmaf(x[i], c, -M));
+      s1 += ex2(fmaf(x[i + 1], c, -M));
+    }
+  }
+  __device__ __forceinline__ void add_one(float x, float c) {
+    raise(x, c);
+    s0 += ex2(fmaf(x, c, -M));
   }
 };
-
-__device__ __forceinline__ void join(float &M, float &s, float M2, float s2) {
-  const float Mx = fmaxf(M, M2);
-  s = s * ex2(M - Mx) + s2 * ex2(M2 - Mx);
-  M = Mx;
-}
 
 struct Scalars {
   float M, k, g;  // gradient: 2^(x c - M) * k, plus g at the id (in the exact path M is the raw maximum)
@@ -163,62 +201,96 @@ struct Sh {
   Scalars row;
 };
 
-// Joins (a, b) over the cluster's threads; every thread of the block gets the
-// result.  `phase` picks how: 0 joins (maximum, sum) pairs, 1 takes the
-// maximum of a, 2 adds b in a fixed order.
-template <int PHASE>
-__device__ float2 cluster_join(Sh &sh, int S, int rank, float a, float b) {
+// The largest of a warp's values, none of them NaN.
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float a2 = __shfl_xor_sync(~0u, a, o), b2 = __shfl_xor_sync(~0u, b, o);
-    if (PHASE == 0) join(a, b, a2, b2);
-    if (PHASE == 1) a = fmaxf(a, a2);
-    if (PHASE == 2) b += b2;
-  }
-  if (PHASE != 0) {  // an earlier join's readers are done
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+  return x;
+}
+// (M, s) pairs of a warp as one: the largest M, and the sums relative to it.
+__device__ __forceinline__ void warp_join(float &M, float &s) {
+  const float top = warp_max(M);
+  s = warp_sum(s * ex2(M - top));
+  M = top;
+}
+
+// Joins (a, b) over the cluster: KIND 0 joins (maximum, sum) pairs, 1 takes
+// the maximum of a, 2 adds b.  Only warp 0 of each CTA gets the result
+// (every lane of it).  `first`: no join of this cluster came before.
+template <int KIND>
+__device__ __forceinline__ float2 cluster_join(Sh &sh, int S, int rank, float a, float b, bool first) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (KIND == 0) warp_join(a, b);
+  if (KIND == 1) a = warp_max(a);
+  if (KIND == 2) b = warp_sum(b);
+  if (!first) {  // an earlier join's readers are done
     if (S == 1)
       __syncthreads();
     else
       cg::this_cluster().sync();
   }
-  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = make_float2(a, b);
+  if (lane == 0) sh.warp[warp] = make_float2(a, b);
   __syncthreads();
-  if (threadIdx.x < (unsigned)S) {  // thread j tells CTA j
-    float2 t = sh.warp[0];
-    for (int w = 1; w < NW; ++w) {
-      const float2 u = sh.warp[w];
-      if (PHASE == 0) join(t.x, t.y, u.x, u.y);
-      if (PHASE == 1) t.x = fmaxf(t.x, u.x);
-      if (PHASE == 2) t.y += u.y;
+  if (warp == 0) {
+    const float2 t = sh.warp[lane & (NW - 1)];  // (each warp's pair on four lanes)
+    a = t.x, b = lane < NW ? t.y : 0.f;
+    if (KIND == 0) warp_join(a, b);
+    if (KIND == 1) a = warp_max(a);
+    if (KIND == 2) b = warp_sum(b);
+    if (S > 1) {
+      if (first) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+      if (lane < S) *cg::this_cluster().map_shared_rank(&sh.cta[rank], lane) = make_float2(a, b);
     }
-    if (S == 1)
-      sh.cta[0] = t;
-    else
-      *cg::this_cluster().map_shared_rank(&sh.cta[rank], threadIdx.x) = t;
+  } else if (S > 1 && first) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   }
-  if (S == 1)
-    __syncthreads();
-  else
+  if (S > 1) {
     cg::this_cluster().sync();
-  float2 t = sh.cta[0];
-  for (int j = 1; j < S; ++j) {
-    const float2 u = sh.cta[j];
-    if (PHASE == 0) join(t.x, t.y, u.x, u.y);
-    if (PHASE == 1) t.x = fmaxf(t.x, u.x);
-    if (PHASE == 2) t.y += u.y;
+    if (warp == 0) {
+      const float2 t = sh.cta[lane & (S - 1)];
+      a = t.x, b = lane < S ? t.y : 0.f;
+      if (KIND == 0) warp_join(a, b);
+      if (KIND == 1) a = warp_max(a);
+      if (KIND == 2) b = warp_sum(b);
+    }
   }
-  return t;
+  return make_float2(a, b);
 }
 
-// The row's scalars in 64 bits, by one thread: xr is the maximum that the
-// sum is relative to.  Every CTA of the row computes them; rank 0 writes them.
+// What a row's loss takes besides its logits, read before the pass over them.
+struct Token {
+  float x, old_logp, ref_logp, adv, weight;
+  template <int MODE>
+  static __device__ __forceinline__ Token read(const Args &a, int row, float x_id) {
+    Token t{x_id, 0.f, 0.f, 0.f, 1.f};
+    if (MODE != LOGPROBS) {
+      t.adv = a.adv[row];
+      if (a.old_logp) t.old_logp = a.old_logp[row];
+      if (a.ref_logp) t.ref_logp = a.ref_logp[row];
+      if (a.weights) t.weight = a.weights[row];
+    }
+    return t;
+  }
+};
+
+// The row's scalars in 64 bits, by a whole warp (its lanes hold the same
+// values; the ratio and the KL term take a lane each): xr is the maximum
+// that the sum s is relative to.  Every CTA of the row computes them; one
+// writes them.
 template <int MODE>
-__device__ Scalars scalars(const Args &a, int row, int64_t id, bool ok, double xr, float s, bool empty, float x_id,
-                           bool writer) {
+__device__ __forceinline__ Scalars scalars(const Args &a, int row, int64_t id, bool ok, double xr, float s, bool empty,
+                                           const Token &tok, bool writer) {
   Scalars r{0.f, 0.f, 0.f, 0};
+  const int lane = threadIdx.x & 31;
   const double ls = log((double)s);
   const double lse = empty ? -INFINITY : xr * a.inv_t + ls;
-  const double lp = !ok ? 0.0 : empty ? -INFINITY : ((double)x_id - xr) * a.inv_t - ls;
+  const double lp = !ok ? 0.0 : empty ? -INFINITY : ((double)tok.x - xr) * a.inv_t - ls;
+  writer = writer && lane == 0;
   if (writer) {
     a.logp[row] = (float)lp;
     if (a.lse) a.lse[row] = (float)lse;
@@ -226,33 +298,81 @@ __device__ Scalars scalars(const Args &a, int row, int64_t id, bool ok, double x
     if (a.status && bits) atomicOr(a.status, bits);
   }
   if (MODE == LOGPROBS) return r;
+  // lane 0: exp(logp - old) - 1, lane 1: exp(ref - logp) - 1
+  const double q = lane == 1 ? (double)tok.ref_logp - lp : a.old_logp ? lp - (double)tok.old_logp : isnan(lp) ? lp : 0.0;
+  const double e = expm1(q);
+  const double ratio = 1.0 + __shfl_sync(~0u, e, 0), eq = __shfl_sync(~0u, e, 1), qq = __shfl_sync(~0u, q, 1);
   double loss = 0.0, d = 0.0;
   if (ok && !empty) {
-    const double A = a.adv[row];
-    const double ratio = a.old_logp ? exp(lp - (double)a.old_logp[row]) : isnan(lp) ? lp : 1.0;
+    const double A = tok.adv;
     const double plain = ratio * A, cut = fmin(fmax(ratio, a.clip_min), a.clip_max) * A;
     loss = -fmin(plain, cut);
     if (isnan(plain)) loss = plain;
     d = plain <= cut ? -plain : isnan(plain) ? plain : 0.0;
     if (a.ref_logp && a.beta != 0.0) {
-      const double q = (double)a.ref_logp[row] - lp, e = expm1(q);
-      loss += a.beta * (q == INFINITY ? q : e - q);
-      d -= a.beta * e;
+      loss += a.beta * (qq == INFINITY ? qq : eq - qq);
+      d -= a.beta * eq;
     }
     if (lp == -INFINITY) d = 0.0;  // an id of probability zero stays there: no gradient
   }
   if (writer) a.loss[row] = (float)loss;
-  const double g = d * (a.weights ? (double)a.weights[row] : 1.0) * a.inv_t;
+  const double g = d * (double)tok.weight * a.inv_t;
   r.g = (float)g;
-  r.k = empty ? 0.f : (float)(-g / (double)s);
+  r.k = empty ? 0.f : -r.g / s;
   return r;
 }
 
-template <typename T, int MODE, bool RESIDENT>
-__global__ void __launch_bounds__(NT) token_rows_kernel(const Args a) {
+// A vector of the gradient, at its place; without 16-byte alignment value by value.
+template <typename T>
+__device__ __forceinline__ void store(T *o, bool vec_out, const float (&x)[Vec<T>::E]) {
+  if (vec_out) {
+    __stcs(reinterpret_cast<uint4 *>(o), Vec<T>::pack(x));
+  } else {
+#pragma unroll
+    for (int i = 0; i < Vec<T>::E; ++i) put(o + i, x[i]);
+  }
+}
+
+// 2^(x c - M) * k over a slice; with `exact`, 2^((x - M) c) * k.  k = 0 (an
+// empty row, or one whose loss does not move with it): zeros, whatever it holds.
+template <typename T, typename Load>
+__device__ __forceinline__ void write_grad(const Row<T> &in, T *out, bool vec_out, int v0, int v1, int fringe,
+                                           float x_fringe, float c, float M, float k, bool exact, Load load) {
   constexpr int E = Vec<T>::E;
-  constexpr int U = 4;  // vectors in flight per thread
-  extern __shared__ __align__(16) uint4 stored[];
+  constexpr int UW = 4;  // vectors in flight per thread
+  T *o = out + in.head;
+  const int first = v0 + (int)threadIdx.x;
+  if (k == 0.f) {
+    if (fringe >= 0) put(out + fringe, 0.f);
+    const float zero[E] = {};
+    for (int v = first; v < v1; v += NT) store<T>(o + v * E, vec_out, zero);
+  } else if (!exact) {
+    if (fringe >= 0) put(out + fringe, ex2(fmaf(x_fringe, c, -M)) * k);
+    each_vector<UW>(first, v1, load, [&](int v, const uint4 &w) {
+      float x[E];
+      Vec<T>::unpack(w, x);
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = ex2(fmaf(x[i], c, -M)) * k;
+      store<T>(o + v * E, vec_out, x);
+    });
+  } else {
+    if (fringe >= 0) put(out + fringe, ex2((x_fringe - M) * c) * k);
+    for (int v = first; v < v1; v += NT) {
+      float x[E];
+      Vec<T>::unpack(load(v), x);
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = ex2((x[i] - M) * c) * k;
+      store<T>(o + v * E, vec_out, x);
+    }
+  }
+}
+
+// (six blocks per SM: 40 registers; without the bound 60, four blocks and 506 in
+// place of 470 us for 4096 rows of 151936 bf16)
+template <typename T, int MODE>
+__global__ void __launch_bounds__(NT, 6) token_rows_kernel(const Args a) {
+  constexpr int E = Vec<T>::E;
+  constexpr int U = 6;  // vectors in flight per thread
   __shared__ Sh sh;
   const int S = a.S, rank = (int)(blockIdx.x % (unsigned)S), row = (int)(blockIdx.x / (unsigned)S);
   const int tid = threadIdx.x;
@@ -285,44 +405,39 @@ __global__ void __launch_bounds__(NT) token_rows_kernel(const Args a) {
     }
     return;
   }
-  if (S > 1) cg::this_cluster().sync();  // a CTA writes into a peer's shared memory only once the peer runs
+  // a CTA writes into a peer's shared memory only once the peer runs: every
+  // CTA arrives here, and waits before it writes
+  if (S > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const float x_id = ok ? to_f(in.p[id]) : 0.f;
+  Token tok{};
+  if (tid < 32) tok = Token::read<MODE>(a, row, x_id);
   const float x_fringe = fringe >= 0 ? to_f(in.p[fringe]) : 0.f;
   const float c = a.c;
   Stat st(c);
-  for (int v = v0 + tid; v < v1; v += NT * U) {
-    uint4 w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * NT < v1) w[u] = __ldcs(in.vecs() + v + u * NT);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * NT < v1) {
-        if (MODE == POLICY_GRAD && RESIDENT) stored[v + u * NT - v0] = w[u];
-        float x[E];
-        Vec<T>::unpack(w[u], x);
-        st.add(x, c);
-      }
+  // (a gradient reads the slice again, from L2: the rows in flight are some
+  // tens of megabytes; otherwise it is read once)
+  each_vector<U>(
+      v0 + tid, v1, [&](int v) { return MODE == POLICY_GRAD ? in.vecs()[v] : __ldcs(in.vecs() + v); },
+      [&](int, const uint4 &w) { st.add<T>(w, c); });
+  if (fringe >= 0) st.add_one(x_fringe, c);
+  float2 t = cluster_join<0>(sh, S, rank, st.M, st.s0 + st.s1, true);
+  if (tid < 32) {
+    Scalars r{};
+    const bool exact = !(t.x > FLOOR * c && t.x < -FLOOR * c);
+    if (!exact) r = scalars<MODE>(a, row, id, ok, (double)t.x / (double)c, t.y, false, tok, rank == 0);
+    r.M = t.x;
+    r.exact = exact;
+    if (tid == 0) sh.row = r;
   }
-  if (fringe >= 0) {
-    const float x[1] = {x_fringe};
-    st.add(x, c);
-  }
-  float2 t = cluster_join<0>(sh, S, rank, st.M, st.s);
-  const bool exact = !(t.x > FLOOR * c && t.x < -FLOOR * c);
-  bool empty = false;
-  auto load = [&](int v) {
-    return MODE == POLICY_GRAD && RESIDENT ? stored[v - v0] : in.vecs()[v];
-  };
-  if (exact) {  // the row's largest value is at the edge of the type (or nothing is left of it)
+  __syncthreads();
+  auto load = [&](int v) { return __ldcs(in.vecs() + v); };
+  if (sh.row.exact) {  // the row's largest value is at the edge of the type (or nothing is left of it)
     float m = fringe >= 0 ? x_fringe : -INFINITY;
-    for (int v = v0 + tid; v < v1; v += NT) {
-      float x[E];
-      Vec<T>::unpack(load(v), x);
-#pragma unroll
-      for (int i = 0; i < E; ++i) m = fmaxf(m, x[i]);
-    }
-    m = cluster_join<1>(sh, S, rank, m, 0.f).x;
+    for (int v = v0 + tid; v < v1; v += NT) m = fmaxf(m, Vec<T>::largest(load(v)));
+    m = cluster_join<1>(sh, S, rank, m, 0.f, false).x;
+    if (tid == 0) sh.row.M = m;
+    __syncthreads();
+    m = sh.row.M;
     float s = fringe >= 0 ? ex2((x_fringe - m) * c) : 0.f;
     for (int v = v0 + tid; v < v1; v += NT) {
       float x[E];
@@ -330,36 +445,26 @@ __global__ void __launch_bounds__(NT) token_rows_kernel(const Args a) {
 #pragma unroll
       for (int i = 0; i < E; ++i) s += ex2((x[i] - m) * c);
     }
-    t = make_float2(m, cluster_join<2>(sh, S, rank, 0.f, s).y);
-    empty = m == -INFINITY;
-  }
-  if (tid == 0) {
-    const double xr = exact ? (double)t.x : (double)t.x / (double)c;
-    Scalars r = scalars<MODE>(a, row, id, ok, xr, t.y, empty, x_id, rank == 0);
-    r.M = t.x;
-    r.exact = exact;
-    sh.row = r;
+    t = cluster_join<2>(sh, S, rank, 0.f, s, false);
+    if (tid < 32) {
+      Scalars r = scalars<MODE>(a, row, id, ok, (double)m, t.y, m == -INFINITY, tok, rank == 0);
+      r.M = m;
+      r.exact = 1;
+      if (tid == 0) sh.row = r;
+    }
+    __syncthreads();
   }
   if (MODE != POLICY_GRAD) return;
-  __syncthreads();
   const Scalars r = sh.row;
-  auto grad = [&](float x, int at) {
-    // (an empty row, or a row whose loss does not move with it: zeros, whatever its logits hold)
-    float y = r.k == 0.f ? 0.f : ex2(r.exact ? (x - r.M) * c : fmaf(x, c, -r.M)) * r.k;
-    return at == (int)id ? y + r.g : y;
-  };
-  if (fringe >= 0) put(out + fringe, grad(x_fringe, fringe));
-  for (int v = v0 + tid; v < v1; v += NT) {
-    float x[E], y[E];
-    Vec<T>::unpack(load(v), x);
-    const int at = in.head + v * E;
-#pragma unroll
-    for (int i = 0; i < E; ++i) y[i] = grad(x[i], at + i);
-    if (vec_out)
-      __stcs(reinterpret_cast<uint4 *>(out + at), Vec<T>::pack(y));
-    else
-#pragma unroll
-      for (int i = 0; i < E; ++i) put(out + at + i, y[i]);
+  write_grad<T>(in, out, vec_out, v0, v1, fringe, x_fringe, c, r.M, r.k, r.exact, load);
+  // the id's own element: its probability's share, plus g
+  const int own = (int)id - in.head;
+  const bool mine = own < 0 ? rank == 0 : own >= in.nv * E ? rank == S - 1 : own >= v0 * E && own < v1 * E;
+  if (!mine) return;
+  __syncthreads();  // the element is written once more, after whoever wrote it
+  if (tid == 0) {
+    const float p = r.k == 0.f ? 0.f : ex2(r.exact ? (x_id - r.M) * c : fmaf(x_id, c, -r.M)) * r.k;
+    put(out + id, p + r.g);
   }
 }
 
@@ -369,7 +474,7 @@ struct GradArgs {
   int32_t N, V, S;
   const int64_t *ids;
   float c;
-  double inv_t;
+  double inv_t, tc;  // 1 / T; T times the rounded c
   const float *lse, *dlogp;
   void *dlogits;
   int64_t ldd;
@@ -381,7 +486,7 @@ struct GradArgs {
 template <typename T>
 __global__ void __launch_bounds__(NT) token_logprobs_grad_kernel(const GradArgs a) {
   constexpr int E = Vec<T>::E;
-  constexpr int U = 4;
+  constexpr int U = 4;  // vectors in flight per thread
   __shared__ float sM, sk, sg;
   const int S = a.S, rank = (int)(blockIdx.x % (unsigned)S), row = (int)(blockIdx.x / (unsigned)S);
   const int tid = threadIdx.x;
@@ -394,41 +499,40 @@ __global__ void __launch_bounds__(NT) token_logprobs_grad_kernel(const GradArgs 
                                                                        : -1;
   const int64_t id = a.ids[row];
   if (tid == 0) {
-    const bool ok = id >= 0 && id < a.V && a.lse[row] != -INFINITY;
-    const double g = ok ? (double)a.dlogp[row] * a.inv_t : 0.0;
-    const double M = (double)a.lse[row] / a.inv_t * (double)a.c;
-    sM = (float)M;
-    sg = (float)g;
-    sk = (float)(-g * exp2((double)(float)M - M));
-    if (!ok) sM = 0.f, sk = 0.f;
+    const float lse = a.lse[row];
+    const bool ok = id >= 0 && id < a.V && lse != -INFINITY;
+    const float g = ok ? (float)((double)a.dlogp[row] * a.inv_t) : 0.f;
+    const double M = (double)lse * a.tc;
+    sM = ok ? (float)M : 0.f;
+    sg = g;
+    sk = ok ? -g * ex2((float)((double)(float)M - M)) : 0.f;
   }
   __syncthreads();
   const float M = sM, k = sk, g = sg, c = a.c;
-  auto grad = [&](float x, int at) {
-    const float y = k == 0.f ? 0.f : ex2(fmaf(x, c, -M)) * k;
-    return at == (int)id ? y + g : y;
-  };
-  if (fringe >= 0) put(out + fringe, grad(to_f(in.p[fringe]), fringe));
-  for (int v = v0 + tid; v < v1; v += NT * U) {
-    uint4 w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * NT < v1) w[u] = __ldcs(in.vecs() + v + u * NT);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * NT < v1) {
-        float x[E], y[E];
-        Vec<T>::unpack(w[u], x);
-        const int at = in.head + (v + u * NT) * E;
-#pragma unroll
-        for (int i = 0; i < E; ++i) y[i] = grad(x[i], at + i);
-        if (vec_out)
-          __stcs(reinterpret_cast<uint4 *>(out + at), Vec<T>::pack(y));
-        else
-#pragma unroll
-          for (int i = 0; i < E; ++i) put(out + at + i, y[i]);
-      }
+  if (fringe >= 0) {
+    const float x = to_f(in.p[fringe]);
+    put(out + fringe, (k == 0.f ? 0.f : ex2(fmaf(x, c, -M)) * k) + (fringe == id ? g : 0.f));
   }
+  const int64_t own = id - in.head;  // where the id lies among the vectors' values
+  const int own_vec = own >= 0 && own < (int64_t)in.nv * E ? (int)(own / E) : -1;
+  T *o = out + in.head;
+  each_vector<U>(
+      v0 + tid, v1, [&](int v) { return __ldcs(in.vecs() + v); },
+      [&](int v, const uint4 &w) {
+        float x[E];
+        Vec<T>::unpack(w, x);
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = ex2(fmaf(x[i], c, -M)) * k;
+        if (k == 0.f) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) x[i] = 0.f;
+        }
+        if (v == own_vec) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) x[i] += own == (int64_t)v * E + i ? g : 0.f;
+        }
+        store<T>(o + v * E, vec_out, x);
+      });
 }
 
 // ------------------------------------------------------------ host side
@@ -461,17 +565,11 @@ static int launched() {
   return e == cudaSuccess ? MSTAR_OK : fail(MSTAR_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e));
 }
 
-template <typename T, int MODE, bool RESIDENT>
-static int launch(const Args &a, int smem, cudaStream_t st) {
-  auto kern = token_rows_kernel<T, MODE, RESIDENT>;
-  if (smem > 48 * 1024 - (int)sizeof(Sh)) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
-  }
+template <typename T, int MODE>
+static int launch(const Args &a, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.N * (unsigned)a.S, 1, 1);
   cfg.blockDim = dim3(NT, 1, 1);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -480,7 +578,7 @@ static int launch(const Args &a, int smem, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_rows_kernel<T, MODE>, a);
   if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e));
   return MSTAR_OK;
 }
@@ -488,11 +586,8 @@ static int launch(const Args &a, int smem, cudaStream_t st) {
 template <typename T>
 static int run(Args &a, int mode, cudaStream_t st) {
   a.S = slices(a.N, (int64_t)a.V * (int)sizeof(T));
-  if (mode == LOGPROBS) return launch<T, LOGPROBS, false>(a, 0, st);
-  if (mode == POLICY) return launch<T, POLICY, false>(a, 0, st);
-  const int64_t vecs = ((int64_t)a.V / Vec<T>::E + a.S - 1) / a.S;
-  if (vecs * 16 <= MAX_RESIDENT) return launch<T, POLICY_GRAD, true>(a, (int)vecs * 16, st);
-  return launch<T, POLICY_GRAD, false>(a, 0, st);
+  if (mode == LOGPROBS) return launch<T, LOGPROBS>(a, st);
+  return mode == POLICY ? launch<T, POLICY>(a, st) : launch<T, POLICY_GRAD>(a, st);
 }
 
 static void set_temperature(double temperature, float &c, double &inv_t) {
@@ -543,12 +638,13 @@ int mstar_token_logprobs_grad(const void *logits, int32_t dtype, int32_t N, int3
   a.V = V;
   a.ids = ids;
   rows::set_temperature(temperature, a.c, a.inv_t);
+  a.tc = temperature * (double)a.c;
   a.lse = lse;
   a.dlogp = dlogp;
   a.dlogits = dlogits;
   a.ldd = ld_dlogits;
   const int es = dtype == MSTAR_DTYPE_F32 ? 4 : 2;
-  const int64_t per = (int64_t)rows::NT * 4 * 16;  // one unrolled step of a block
+  const int64_t per = (int64_t)rows::NT * 4 * 16 * 4;  // four unrolled steps of a block
   a.S = (int)std::max<int64_t>(1, ((int64_t)V * es + per - 1) / per);
   while (a.S > 1 && (int64_t)N * a.S > 0x7FFFFFFF) a.S = (a.S + 1) / 2;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
