@@ -11,15 +11,18 @@
 // Gradient: the tokens are sorted by id first, so each row of the table is
 // summed by one owner in position order (no atomics on values: the same
 // inputs give the same bits) and every row of the output is written once.
-//   sort   each CTA takes a range of ids and reads all ids twice: once to
-//          count (per id and per warp, each warp owning a contiguous part of
-//          the positions), once to place.  It counts the ids below its range
-//          as it goes, so CTAs need nothing of one another.
+//   sort   CTA c of C (a power of two) takes the ids v with v mod C = c, which
+//          spreads frequent neighbours, and reads all ids twice: once to count
+//          (per id and per warp, each warp owning a contiguous part of the
+//          positions), once to place.  It counts the ids of the CTAs before it
+//          as it goes, so CTAs need nothing of one another.  The order of the
+//          ids is then (v mod C, v / C); all that matters is that an id's
+//          tokens lie together, in position order.
 //   sums   the sorted positions in chunks of equal length, whatever the ids'
-//          frequencies; runs inside a chunk are written, runs that cross a
-//          border leave 32-bit partial sums.  Further CTAs of the same launch
+//          frequencies; a chunk writes the runs that start in it, and long runs
+//          that cross its borders leave 32-bit partial sums.  Further CTAs of the same launch
 //          write the rows that no token has.
-//   joins  the chunk in which a crossing run starts adds its parts in order.
+//   joins  the parts of each long run that crosses borders are added in order.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -191,8 +194,13 @@ __global__ void __launch_bounds__(NT) embed_w4_kernel(const Lookup a) {
 
 constexpr int SORT_NT = 1024;
 constexpr int SORT_NW = SORT_NT / 32;
-constexpr int MAX_BINS = 1088;  // ids per CTA of the sort: 156940 ids fit 148 CTAs
+constexpr int SORT_U = 16;       // ids per lane and step
+constexpr int MAX_BINS = SORT_NT;  // ids per CTA of the sort
 constexpr int SUM_NT = 128;
+constexpr int JOIN_G = 8;
+constexpr int MAX_CHUNK = 128;
+constexpr int LONG_RUN = 32;  // a run of at most this many tokens belongs to the chunk in which it starts
+constexpr int ZERO_ROWS = 32;
 
 struct Grad {
   const void *dout;
@@ -203,187 +211,250 @@ struct Grad {
   const void *base;  // [V, d] of the output's type, or NULL
   void *out;         // [V, d]
   uint32_t *status;
-  int32_t bins;      // ids per CTA of the sort
-  int32_t chunk, nchunks, col_tiles, zero_rows, nzero;
-  int32_t *start;    // [V + 1] first sorted place of each id
+  int32_t bins, c_log2;  // ids per CTA of the sort, and how many CTAs
+  int32_t chunk, nchunks, col_tiles;
+  int32_t *start;    // [C * bins + 1] first sorted place of each id, in the sort's order of ids
   int32_t *pos;      // [N] positions, sorted by id, then by position
   int32_t *key;      // [N] their ids
   float *part;       // [nchunks][2][d]: a run from the chunk before / into the chunk after
 };
 
+// An id's place in the sort's order.
+__device__ __forceinline__ int rank_of(const Grad &a, int v) {
+  return (v & ((1 << a.c_log2) - 1)) * a.bins + (v >> a.c_log2);
+}
+
 __global__ void __launch_bounds__(SORT_NT) sort_tokens_kernel(const Grad a) {
-  extern __shared__ int32_t cnt[];  // [SORT_NW][bins]
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(16) int32_t cnt[];  // [SORT_NW][bins]
   __shared__ int32_t below_w[SORT_NW], scan_w[SORT_NW];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int base = (int)blockIdx.x * a.bins, bins = min(a.bins, a.V - base);
-  for (int i = tid; i < SORT_NW * a.bins; i += SORT_NT) cnt[i] = 0;
+  const int me = (int)blockIdx.x, mask = (1 << a.c_log2) - 1;
+  for (int i = tid; i < SORT_NW * a.bins / 4; i += SORT_NT) reinterpret_cast<int4 *>(cnt)[i] = make_int4(0, 0, 0, 0);
   __syncthreads();
   const int n0 = (int)((int64_t)a.N * warp / SORT_NW), n1 = (int)((int64_t)a.N * (warp + 1) / SORT_NW);
   int32_t *mine = cnt + warp * a.bins;
-  int below = 0;
+  int id[SORT_U];  // -1: none, or not in the table
   bool bad = false;
-  constexpr int U = 8;
-  for (int n = n0 + lane; n < n1; n += 32 * U) {
-    int64_t id[U];
+  auto load_ids = [&](int n) {
+    int64_t x[SORT_U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) id[u] = n + 32 * u < n1 ? __ldg(a.ids + n + 32 * u) : -1;
+    for (int u = 0; u < SORT_U; ++u) x[u] = n + 32 * u < n1 ? __ldg(a.ids + n + 32 * u) : -1;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      below += id[u] >= 0 && id[u] < base;
-      bad |= id[u] >= a.V;
-      if (id[u] >= base && id[u] < base + bins) atomicAdd(&mine[(int)id[u] - base], 1);
+    for (int u = 0; u < SORT_U; ++u) {
+      bad |= x[u] >= a.V;
+      id[u] = x[u] >= 0 && x[u] < a.V ? (int)x[u] : -1;
+    }
+  };
+  int below = 0;
+  for (int nb = n0; nb < n1; nb += 32 * SORT_U) {  // (the same steps for every lane: each gets its ids, or -1)
+    load_ids(nb + lane);
+#pragma unroll
+    for (int u = 0; u < SORT_U; ++u) {
+      const int c = id[u] & mask;
+      below += id[u] >= 0 && c < me;
+      if (id[u] >= 0 && c == me) atomicAdd(&mine[id[u] >> a.c_log2], 1);
     }
   }
-  if (bad && blockIdx.x == 0 && a.status) atomicOr(a.status, MSTAR_STATUS_BAD_ID);
-  for (int o = 16; o; o >>= 1) below += __shfl_xor_sync(~0u, below, o);
+  if (bad && me == 0 && a.status) atomicOr(a.status, MSTAR_STATUS_BAD_ID);
+  below = __reduce_add_sync(~0u, below);
   if (lane == 0) below_w[warp] = below;
   __syncthreads();
-  int first = 0;
-  for (int w = 0; w < SORT_NW; ++w) first += below_w[w];
-  // exclusive prefix over the ids, then over the warps of each id
-  for (int b0 = 0; b0 < bins; b0 += SORT_NT) {
-    const int b = b0 + tid;
-    int tot = 0;
-    if (b < bins)
-      for (int w = 0; w < SORT_NW; ++w) tot += cnt[w * a.bins + b];
-    int inc = tot;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(~0u, inc, o);
-      if (lane >= o) inc += t;
-    }
-    if (lane == 31) scan_w[warp] = inc;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < SORT_NW; ++w) {
-      if (w < warp) before += scan_w[w];
-      all += scan_w[w];
-    }
-    int at = first + before + inc - tot;
-    if (b < bins) {
-      a.start[base + b] = at;
-      for (int w = 0; w < SORT_NW; ++w) {
-        const int t = cnt[w * a.bins + b];
-        cnt[w * a.bins + b] = at;
-        at += t;
+  // exclusive prefix over the ids (a thread each), then over the warps of each id
+  int tot = 0;
+  if (tid < a.bins)
+    for (int w = 0; w < SORT_NW; ++w) tot += cnt[w * a.bins + tid];
+  int inc = tot;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(~0u, inc, o);
+    if (lane >= o) inc += t;
+  }
+  if (lane == 31) scan_w[warp] = inc;
+  __syncthreads();
+  const int first = __reduce_add_sync(~0u, below_w[lane]);
+  const int before = __reduce_add_sync(~0u, lane < warp ? scan_w[lane] : 0);
+  const int all = __reduce_add_sync(~0u, scan_w[lane]);
+  int at = first + before + inc - tot;
+  if (tid < a.bins) {
+    a.start[me * a.bins + tid] = at;
+    for (int w0 = 0; w0 < SORT_NW; w0 += 8) {
+      int t[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) t[w] = cnt[(w0 + w) * a.bins + tid];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        cnt[(w0 + w) * a.bins + tid] = at;
+        at += t[w];
       }
     }
-    first += all;
-    __syncthreads();
   }
-  if (tid == 0 && base + bins == a.V) a.start[a.V] = first;
-  for (int nb = n0; nb < n1; nb += 32 * U) {
-    int64_t id[U];
+  if (tid == 0 && me == mask) a.start[(mask + 1) * a.bins] = first + all;
+  __syncthreads();
+  const bool kept = n1 - n0 <= 32 * SORT_U;  // the counting step's ids are still here
+  for (int nb = n0; nb < n1; nb += 32 * SORT_U) {
+    if (!kept) load_ids(nb + lane);
 #pragma unroll
-    for (int u = 0; u < U; ++u) id[u] = nb + 32 * u + lane < n1 ? __ldg(a.ids + nb + 32 * u + lane) : -1;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = id[u] >= base && id[u] < base + bins;
-      const unsigned any = __ballot_sync(~0u, in);
-      if (!any) continue;
-      const int b = in ? (int)id[u] - base : -1;
+    for (int u = 0; u < SORT_U; ++u) {
+      const bool in = id[u] >= 0 && (id[u] & mask) == me;
+      if (!__any_sync(~0u, in)) continue;
+      const int b = in ? id[u] >> a.c_log2 : -1;
       const unsigned same = __match_any_sync(~0u, b);
       const int rank = __popc(same & ((1u << lane) - 1u));
-      int at = 0;
-      if (in) at = mine[b] + rank;
+      int to = 0;
+      if (in) to = mine[b] + rank;
       __syncwarp();
-      if (in && rank == 0) mine[b] = at + __popc(same);
+      if (in && rank == 0) mine[b] = to + __popc(same);
       __syncwarp();
       if (in) {
-        a.pos[at] = nb + 32 * u + lane;
-        a.key[at] = (int)id[u];
+        a.pos[to] = nb + 32 * u + lane;
+        a.key[to] = id[u];
       }
     }
   }
 }
 
 template <typename TO, int W>
-__device__ __forceinline__ void finish(const Grad &a, int v, int col, float (&acc)[W]) {
-  const int64_t at = (int64_t)v * a.d + col;
+__device__ __forceinline__ void load_base(const Grad &a, int v, int col, float (&b)[W]) {
+  if (a.base) load<W>(static_cast<const TO *>(a.base) + (int64_t)v * a.d + col, b);
+}
+template <typename TO, int W>
+__device__ __forceinline__ void finish(const Grad &a, int v, int col, float (&acc)[W], const float (&b)[W]) {
 #pragma unroll
   for (int j = 0; j < W; ++j) acc[j] *= a.scale;
   if (a.base) {
-    float b[W];
-    load<W>(static_cast<const TO *>(a.base) + at, b);
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[j] += b[j];
   }
-  store<W>(static_cast<TO *>(a.out) + at, acc);
+  store<W>(static_cast<TO *>(a.out) + (int64_t)v * a.d + col, acc);
 }
 
 template <typename TI, typename TO, int W>
 __global__ void __launch_bounds__(SUM_NT) sum_tokens_kernel(const Grad a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int work = a.nchunks * a.col_tiles;
+  __shared__ int32_t skey[MAX_CHUNK + LONG_RUN + 2], spos[MAX_CHUNK + LONG_RUN];
   if ((int)blockIdx.x >= work) {  // rows without a token: zeros, or the base's own
-    const int r0 = ((int)blockIdx.x - work) * a.zero_rows;
-    for (int v = r0; v < min(a.V, r0 + a.zero_rows); ++v) {
-      if (a.start[v + 1] > a.start[v]) continue;
+    const int r0 = ((int)blockIdx.x - work) * ZERO_ROWS, rows = min(ZERO_ROWS, a.V - r0);
+    if ((int)threadIdx.x < rows) {
+      const int k = rank_of(a, r0 + (int)threadIdx.x);
+      skey[threadIdx.x] = a.start[k + 1] - a.start[k];
+    }
+    __syncthreads();
+    for (int r = 0; r < rows; ++r) {
+      if (skey[r]) continue;
       for (int col = (int)threadIdx.x * W; col < a.d; col += SUM_NT * W) {
-        float acc[W] = {};
-        finish<TO, W>(a, v, col, acc);
+        float acc[W] = {}, b[W];
+        load_base<TO, W>(a, r0 + r, col, b);
+        finish<TO, W>(a, r0 + r, col, acc, b);
       }
     }
     return;
   }
   const int c = (int)blockIdx.x / a.col_tiles;
   const int col = (((int)blockIdx.x % a.col_tiles) * SUM_NT + (int)threadIdx.x) * W;
-  const int total = a.start[a.V];
+  const int total = a.start[a.bins << a.c_log2];
   const int s0 = c * a.chunk, s1 = min(total, s0 + a.chunk);
-  if (col >= a.d || s0 >= s1) return;
+  if (s0 >= s1) return;
+  // the chunk's ids and positions first, so that the rows' loads wait for nothing
+  const int seen = min(total, s1 + LONG_RUN) - s0;  // tokens that may be this chunk's
+  for (int i = (int)threadIdx.x; i < seen + 2; i += SUM_NT) {
+    const int s = s0 - 1 + i;
+    skey[i] = s >= 0 && s < total ? a.key[s] : -1;
+    if (i < seen) spos[i] = a.pos[s0 + i];
+  }
+  __syncthreads();
+  bool from_before = skey[0] == skey[1];
+  int begin = 0, end = s1 - s0;
+  if (from_before) {  // a short run that started before is not this chunk's
+    const int r = rank_of(a, skey[1]), stop = a.start[r + 1];
+    if (stop - a.start[r] <= LONG_RUN) begin = stop - s0, from_before = false;
+  }
+  if (begin >= end) return;
+  if (skey[end] == skey[end + 1]) {  // a short run that goes on behind is
+    const int r = rank_of(a, skey[end]), stop = a.start[r + 1];
+    if (stop - a.start[r] <= LONG_RUN) end = stop - s0;
+  }
+  if (col >= a.d) return;
   constexpr int U = 4;
-  float acc[W] = {};
-  bool from_before = s0 > 0 && a.key[s0 - 1] == a.key[s0];
-  for (int s = s0; s < s1; s += U) {
+  float acc[W] = {}, b[W];
+  load_base<TO, W>(a, skey[begin + 1], col, b);  // (read as a run begins: it is there when the run ends)
+  for (int s = begin; s < end; s += U) {
     float x[U][W];
-    int key[U + 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s + u < end) load<W>(static_cast<const TI *>(a.dout) + (int64_t)spos[s + u] * a.ldo + col, x[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      key[u] = s + u < s1 ? a.key[s + u] : -1;
-      if (s + u < s1) load<W>(static_cast<const TI *>(a.dout) + (int64_t)a.pos[s + u] * a.ldo + col, x[u]);
-    }
-    key[U] = s + U < total ? a.key[s + U] : -1;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (s + u >= s1) break;
+      if (s + u >= end) break;
 #pragma unroll
       for (int j = 0; j < W; ++j) acc[j] += x[u][j];
-      const int next = s + u + 1 < total ? (s + u + 1 < s1 || u + 1 == U ? key[u + 1] : a.key[s + u + 1]) : -1;
-      const bool last = s + u + 1 == s1;
-      if (next == key[u] && !last) continue;
-      if (from_before || next == key[u]) {  // the run crosses a border of the chunk
-        float *p = a.part + ((int64_t)c * 2 + (from_before ? 0 : 1)) * a.d + col;
-#pragma unroll
-        for (int j = 0; j < W; ++j) p[j] = acc[j];
+      const int key = skey[s + u + 1];
+      const bool goes_on = skey[s + u + 2] == key;
+      if (goes_on && s + u + 1 < end) continue;
+      if (from_before || goes_on) {  // the run crosses a border of the chunk
+        store<W>(a.part + ((int64_t)c * 2 + (from_before ? 0 : 1)) * a.d + col, acc);
       } else {
-        finish<TO, W>(a, key[u], col, acc);
+        finish<TO, W>(a, key, col, acc, b);
       }
       from_before = false;
 #pragma unroll
       for (int j = 0; j < W; ++j) acc[j] = 0.f;
+      if (s + u + 1 < end) load_base<TO, W>(a, skey[s + u + 2], col, b);
     }
   }
 }
 
+// CTA i looks at the borders i, i + grid, ... for runs that start before and go
+// on behind; JOIN_G groups of threads take such a run's parts in turn (a
+// frequent id's run has a hundred), and the first adds the groups' sums in
+// their order.
 template <typename TO, int W>
-__global__ void __launch_bounds__(SUM_NT) join_tokens_kernel(const Grad a) {
-  const int c = (int)blockIdx.x / a.col_tiles;
-  const int col = (((int)blockIdx.x % a.col_tiles) * SUM_NT + (int)threadIdx.x) * W;
-  const int total = a.start[a.V];
-  const int s1 = (c + 1) * a.chunk;  // the border behind this chunk
-  if (col >= a.d || s1 >= total) return;
-  const int id = a.key[s1 - 1];
-  if (a.key[s1] != id || a.start[id] < c * a.chunk) return;  // no run crosses it, or one that starts before
-  const int last = (a.start[id + 1] - 1) / a.chunk;          // the chunk in which it ends
-  float acc[W];
-  const float *p = a.part + ((int64_t)c * 2 + 1) * a.d + col;
+__global__ void __launch_bounds__(SUM_NT *JOIN_G) join_tokens_kernel(const Grad a) {
+  __shared__ float sums[JOIN_G][SUM_NT * W];
+  __shared__ int found[SUM_NT * JOIN_G], nfound;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = (int)threadIdx.x % SUM_NT, group = (int)threadIdx.x / SUM_NT;
+  const int col = ((int)blockIdx.y * SUM_NT + lane) * W;
+  const int total = a.start[a.bins << a.c_log2];
+  const int full = (total - 1) / a.chunk;  // chunks with tokens behind their border
+  for (int c0 = (int)blockIdx.x; c0 < full; c0 += (int)gridDim.x * SUM_NT * JOIN_G) {
+    __syncthreads();
+    if (threadIdx.x == 0) nfound = 0;
+    __syncthreads();
+    const int mine = c0 + (int)threadIdx.x * (int)gridDim.x;
+    if (mine < full) {
+      const int s1 = (mine + 1) * a.chunk, id = a.key[s1 - 1], r = rank_of(a, id), first = a.start[r];
+      if (a.key[s1] == id && first >= mine * a.chunk && a.start[r + 1] - first > LONG_RUN) found[atomicAdd(&nfound, 1)] = mine;
+    }
+    __syncthreads();
+    for (int f = 0; f < nfound; ++f) {  // (their order does not matter: each is an id of its own)
+      const int c = found[f], id = a.key[(c + 1) * a.chunk - 1];
+      const int last = (a.start[rank_of(a, id) + 1] - 1) / a.chunk;  // the chunk in which it ends
+      float acc[W] = {}, b[W];
+      if (col < a.d) {
+        if (group == 0) load_base<TO, W>(a, id, col, b);
+        // part 0 is this chunk's end of the run, part k > 0 chunk c + k's beginning
+#pragma unroll 4
+        for (int k = group; k <= last - c; k += JOIN_G) {
+          float x[W];
+          load<W>(a.part + ((int64_t)(c + k) * 2 + (k == 0 ? 1 : 0)) * a.d + col, x);
 #pragma unroll
-  for (int j = 0; j < W; ++j) acc[j] = p[j];
-#pragma unroll 8
-  for (int k = c + 1; k <= last; ++k) {
-    const float *q = a.part + (int64_t)k * 2 * a.d + col;
+          for (int j = 0; j < W; ++j) acc[j] += x[j];
+        }
+      }
+      __syncthreads();  // the run before has been added
 #pragma unroll
-    for (int j = 0; j < W; ++j) acc[j] += q[j];
+      for (int j = 0; j < W; ++j) sums[group][lane + j * SUM_NT] = acc[j];
+      __syncthreads();
+      if (group == 0 && col < a.d) {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+          for (int k = 1; k < JOIN_G; ++k) acc[j] += sums[k][lane + j * SUM_NT];
+        finish<TO, W>(a, id, col, acc, b);
+      }
+    }
   }
-  finish<TO, W>(a, id, col, acc);
 }
 
 // ------------------------------------------------------------ host side
@@ -433,7 +504,16 @@ static int launch_lookup(const Lookup &a, int w, cudaStream_t st) {
   return launched();
 }
 
-// Workspace: start [V + 1], pos [N], key [N], part [nchunks][2][d], each
+// CTAs of the sort: a power of two that leaves each at most MAX_BINS ids, and
+// enough of them to fill the GPU.
+static int sort_log2(int V) {
+  int l = 7;
+  while (((V + (1 << l) - 1) >> l) > MAX_BINS) ++l;
+  return l;
+}
+static int sort_bins(int V) { return (((V + (1 << sort_log2(V)) - 1) >> sort_log2(V)) + 3) / 4 * 4; }
+
+// Workspace: start [C * bins + 1], pos [N], key [N], part [nchunks][2][d], each
 // rounded to 256 bytes.
 struct Layout {
   int chunk, nchunks, cols;
@@ -443,11 +523,11 @@ static Layout layout(int N, int V, int d) {
   Layout l{};
   // chunks long enough to amortise a border, short enough for some waves of CTAs
   const int64_t tiles = (d + SUM_NT * 8 - 1) / (SUM_NT * 8);
-  l.chunk = (int)std::min<int64_t>(128, std::max<int64_t>(8, (int64_t)N * tiles / (148 * 8)));
+  l.chunk = (int)std::min<int64_t>(MAX_CHUNK, std::max<int64_t>(16, (int64_t)N * tiles / (148 * 16)));
   l.nchunks = (N + l.chunk - 1) / l.chunk;
   const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
   l.start = 0;
-  l.pos = up(((int64_t)V + 1) * 4);
+  l.pos = up((((int64_t)sort_bins(V) << sort_log2(V)) + 1) * 4);
   l.key = l.pos + up((int64_t)N * 4);
   l.part = l.key + up((int64_t)N * 4);
   l.bytes = l.part + up((int64_t)l.nchunks * 2 * d * 4);
@@ -457,23 +537,31 @@ static Layout layout(int N, int V, int d) {
 template <typename TI, typename TO, int W>
 static int launch_grad(Grad &a, cudaStream_t st) {
   a.col_tiles = (a.d + SUM_NT * W - 1) / (SUM_NT * W);
-  const int grid = (a.V + a.bins - 1) / a.bins;
   const int smem = SORT_NW * a.bins * 4;
   cudaError_t e = cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
-  sort_tokens_kernel<<<grid, SORT_NT, smem, st>>>(a);
+  sort_tokens_kernel<<<1 << a.c_log2, SORT_NT, smem, st>>>(a);
   int rc = launched();
   if (rc) return rc;
   const int64_t work = (int64_t)a.nchunks * a.col_tiles;
-  const bool in_place = a.base == a.out;
-  a.nzero = in_place ? 0 : (a.V + a.zero_rows - 1) / a.zero_rows;
-  sum_tokens_kernel<TI, TO, W><<<(unsigned)(work + a.nzero), SUM_NT, 0, st>>>(a);
-  if ((rc = launched())) return rc;
-  if (a.nchunks > 1) {
-    join_tokens_kernel<TO, W><<<(unsigned)work, SUM_NT, 0, st>>>(a);
-    rc = launched();
+  const int nzero = a.base == a.out ? 0 : (a.V + ZERO_ROWS - 1) / ZERO_ROWS;
+  // the next kernels may be placed while the one before ends; they wait for it before they read
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(work + nzero), 1, 1);
+  cfg.blockDim = dim3(SUM_NT, 1, 1);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, sum_tokens_kernel<TI, TO, W>, a);
+  if (e == cudaSuccess && a.nchunks > 1) {
+    cfg.gridDim = dim3((unsigned)std::min(a.nchunks - 1, 148), (unsigned)a.col_tiles, 1);
+    cfg.blockDim = dim3(SUM_NT * JOIN_G, 1, 1);
+    e = cudaLaunchKernelEx(&cfg, join_tokens_kernel<TO, W>, a);
   }
-  return rc;
+  return e == cudaSuccess ? MSTAR_OK : fail(MSTAR_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e));
 }
 
 template <typename TI, typename TO>
@@ -580,11 +668,10 @@ int mstar_embed_tokens_grad(const int64_t *ids, int32_t N, const void *dout, int
   a.base = base;
   a.out = out;
   a.status = status;
-  // equal ranges, one per SM where the table allows it
-  a.bins = std::min(emb::MAX_BINS, (V + sm_count() - 1) / sm_count());
+  a.bins = emb::sort_bins(V);
+  a.c_log2 = emb::sort_log2(V);
   a.chunk = l.chunk;
   a.nchunks = l.nchunks;
-  a.zero_rows = 8;
   a.start = reinterpret_cast<int32_t *>(ws + l.start);
   a.pos = reinterpret_cast<int32_t *>(ws + l.pos);
   a.key = reinterpret_cast<int32_t *>(ws + l.key);
