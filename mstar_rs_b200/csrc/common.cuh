@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -73,6 +74,22 @@ int fail(int code, const std::string &msg);  // keeps `msg` for mstar_sampler_la
 int current_device();
 int sm_count();
 int max_smem_optin();
+
+// Lets kernel K use `bytes` of dynamic shared memory on the current device;
+// the runtime is asked once per device and larger size.
+template <auto K>
+inline int allow_smem(int bytes) {
+  static std::atomic<int> allowed[kMaxDevices];
+  std::atomic<int> &have = allowed[current_device()];
+  if (have.load(std::memory_order_relaxed) >= bytes) return MSTAR_OK;
+  const cudaError_t e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+  int old = have.load(std::memory_order_relaxed);
+  while (old < bytes && !have.compare_exchange_weak(old, bytes)) {
+  }
+  return MSTAR_OK;
+}
+
 int check_w4(const mstar_w4_t *w);  // a 4-bit matrix's sizes and pointers (w4head.cu)
 
 }  // namespace mstar

@@ -538,11 +538,10 @@ template <typename TI, typename TO, int W>
 static int launch_grad(Grad &a, cudaStream_t st) {
   a.col_tiles = (a.d + SUM_NT * W - 1) / (SUM_NT * W);
   const int smem = SORT_NW * a.bins * 4;
-  cudaError_t e = cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
-  sort_tokens_kernel<<<1 << a.c_log2, SORT_NT, smem, st>>>(a);
-  int rc = launched();
+  int rc = allow_smem<sort_tokens_kernel>(smem);
   if (rc) return rc;
+  sort_tokens_kernel<<<1 << a.c_log2, SORT_NT, smem, st>>>(a);
+  if ((rc = launched())) return rc;
   const int64_t work = (int64_t)a.nchunks * a.col_tiles;
   const int nzero = a.base == a.out ? 0 : (a.V + ZERO_ROWS - 1) / ZERO_ROWS;
   // the next kernels may be placed while the one before ends; they wait for it before they read
@@ -555,7 +554,7 @@ static int launch_grad(Grad &a, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, sum_tokens_kernel<TI, TO, W>, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, sum_tokens_kernel<TI, TO, W>, a);
   if (e == cudaSuccess && a.nchunks > 1) {
     cfg.gridDim = dim3((unsigned)std::min(a.nchunks - 1, 148), (unsigned)a.col_tiles, 1);
     cfg.blockDim = dim3(SUM_NT * JOIN_G, 1, 1);

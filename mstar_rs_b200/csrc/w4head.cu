@@ -837,8 +837,8 @@ template <int N, int GPB>
 static int launch(const CUtensorMap &tw, const CUtensorMap &th, const Gemm &g, cudaStream_t st) {
   auto kern = w4_gemm_kernel<N, GPB>;
   const int smem = g.wstages * W_BYTES + g.hstages * g.n * KB * 2 + 1024;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+  const int rc = allow_smem<w4_gemm_kernel<N, GPB>>(smem);
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid_of(g), 1, 1);
   cfg.blockDim = dim3(Roles<N>::THREADS, 1, 1);
@@ -849,7 +849,7 @@ static int launch(const CUtensorMap &tw, const CUtensorMap &th, const Gemm &g, c
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, tw, th, g);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, th, g);
   if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("launch: ") + cudaGetErrorString(e));
   return MSTAR_OK;
 }

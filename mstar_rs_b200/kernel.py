@@ -9,6 +9,7 @@ validated here (before any launch) and again by the C ABI.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -368,18 +369,29 @@ def lmhead_step(hidden: torch.Tensor, weight: torch.Tensor, logits: torch.Tensor
 # ------------------------------------------------- 4-bit weights, lookup, log-probabilities, policy loss
 
 _ES = {torch.float32: 4, torch.bfloat16: 2}
+_FN: dict = {}  # entry points by name, once the library is loaded
 
 
 def _call(dev: torch.device, name: str, *args) -> None:
     """Entry point `name` with `args` and the current stream of `dev`, on `dev`."""
-    fn = getattr(N.lib(), name)
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(N.lib(), name)
     if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = fn(*args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _raw_stream(dev.index))
     if rc != N.OK:
         N.check(rc, name)
+
+
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without the Stream object around it
+    _raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811
 
 
 def _cuda(t: torch.Tensor, name: str) -> torch.device:
@@ -392,13 +404,13 @@ def _vec(t, name, dtype, dev, n):
     """The address of a contiguous [n] tensor of `dtype` (None: NULL)."""
     if t is None:
         return None
+    if t.dtype is dtype and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() and t.device == dev:
+        return t.data_ptr()
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != dev:
         raise ValueError(f"{name} must live on {dev}, got {t.device}")
-    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous [{n}] tensor, got shape {tuple(t.shape)}")
-    return t.data_ptr()
+    raise ValueError(f"{name} must be a contiguous [{n}] tensor, got shape {tuple(t.shape)}")
 
 
 def _status(t, dev):
@@ -411,6 +423,9 @@ def _status(t, dev):
 
 def _matrix(t, name, dev, rows, cols):
     """Checks a [rows, cols] float32 / bfloat16 matrix with contiguous rows."""
+    if t.dtype in _DT and t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols and t.is_contiguous() \
+            and t.device == dev:
+        return
     if t.dtype not in _DT:
         raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
     if t.device != dev:
@@ -473,14 +488,12 @@ def _w4(codes, scales, zeros) -> N.W4:
     G = scales.shape[1]
     if G < 1 or d % G or d // G not in (32, 64, 128):
         raise ValueError(f"scales give groups of {d / max(G, 1):g} columns; they must be of 32, 64 or 128")
-    w = N.W4()
+    zp = None
     if zeros is not None:
         if zeros.dtype != torch.uint8 or zeros.device != dev or zeros.shape != scales.shape or not zeros.is_contiguous():
             raise ValueError("zeros must be a contiguous uint8 tensor of the scales' shape on their device")
-        w.zeros = zeros.data_ptr()
-    w.codes, w.scales = codes.data_ptr(), scales.data_ptr()
-    w.V, w.d, w.group, w.scale_dtype = V, d, d // G, _DT[scales.dtype]
-    return w
+        zp = zeros.data_ptr()
+    return N.W4(codes.data_ptr(), scales.data_ptr(), zp, V, d, d // G, _DT[scales.dtype])
 
 
 def _check_hidden_w4(hidden, w, dev):
@@ -493,15 +506,21 @@ def _check_hidden_w4(hidden, w, dev):
     return B
 
 
+@functools.lru_cache(maxsize=256)
+def _w4_workspace_bytes(B: int, V: int, d: int, index: int) -> int:
+    with torch.cuda.device(index):
+        n = int(N.lib().mstar_lmhead_w4_workspace_bytes(B, V, d))
+    if n <= 0:
+        N.check(N.ERR_INVALID, "mstar_lmhead_w4_workspace_bytes")
+    return n
+
+
 def lmhead_w4_workspace(B: int, V: int, d: int, device) -> torch.Tensor:
     """Scratch for lmhead_logits_w4 calls of these sizes
     (mstar_lmhead_w4_workspace_bytes); calls that share it must not overlap."""
     dev = torch.device(device)
-    with torch.cuda.device(dev):
-        n = int(N.lib().mstar_lmhead_w4_workspace_bytes(B, V, d))
-    if n <= 0:
-        N.check(N.ERR_INVALID, "mstar_lmhead_w4_workspace_bytes")
-    return torch.empty(n, dtype=torch.uint8, device=dev)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    return torch.empty(_w4_workspace_bytes(B, V, d, index), dtype=torch.uint8, device=torch.device("cuda", index))
 
 
 def lmhead_logits_w4(hidden: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, zeros=None,
@@ -522,7 +541,7 @@ def lmhead_logits_w4(hidden: torch.Tensor, codes: torch.Tensor, scales: torch.Te
     else:
         _matrix(out, "out", dev, B, w.V)
     if workspace is None:
-        workspace = lmhead_w4_workspace(B, w.V, w.d, dev)
+        workspace = torch.empty(_w4_workspace_bytes(B, w.V, w.d, dev.index), dtype=torch.uint8, device=dev)
     wp, wn = _check_ws(workspace, dev)
     _call(dev, "mstar_lmhead_logits_w4", hidden.data_ptr(), _ld(hidden), B, ctypes.byref(w), out.data_ptr(),
           _DT[out.dtype], _ld(out), wp, wn, _status(status, dev))
@@ -606,6 +625,14 @@ def embed_tokens_w4(ids: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _embed_grad_workspace_bytes(n: int, V: int, d: int) -> int:
+    nbytes = int(N.lib().mstar_embed_grad_workspace_bytes(n, V, d))
+    if nbytes <= 0:
+        raise ValueError(f"N={n}, V={V}, d={d} are outside [1, 2^24], [1, 2^21], [1, 65536]")
+    return nbytes
+
+
 def embed_tokens_grad(ids: torch.Tensor, dout: torch.Tensor, V: int, *, scale: float = 1.0,
                       base: torch.Tensor | None = None, out: torch.Tensor | None = None, dtype=None,
                       status: torch.Tensor | None = None) -> torch.Tensor:
@@ -642,9 +669,7 @@ def embed_tokens_grad(ids: torch.Tensor, dout: torch.Tensor, V: int, *, scale: f
         if base is None:
             return out.zero_()
         return out if base.data_ptr() == out.data_ptr() else out.copy_(base)
-    nbytes = int(N.lib().mstar_embed_grad_workspace_bytes(n, V, d))
-    if nbytes <= 0:
-        raise ValueError(f"N={n}, V={V}, d={d} are outside [1, 2^24], [1, 2^21], [1, 65536]")
+    nbytes = _embed_grad_workspace_bytes(n, V, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call(dev, "mstar_embed_tokens_grad", ids.data_ptr(), n, dout.data_ptr(), _DT[dout.dtype], _ld(dout), V, d, scale,
           None if base is None else base.data_ptr(), out.data_ptr(), _DT[out.dtype], ws.data_ptr(), nbytes, st)
@@ -727,15 +752,13 @@ def policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logp: torch.Tensor 
     row: loss 0, logp 0, a zero gradient, and its logits are not read."""
     dev, n, V, ip = _check_rows(logits, ids, temperature)
     f32 = torch.float32
-    p = N.PolicyParams()
-    p.ids = ip
-    p.old_logp = _vec(old_logp, "old_logp", f32, dev, n)
-    p.ref_logp = _vec(ref_logp, "ref_logp", f32, dev, n)
-    p.advantages = _vec(advantages, "advantages", f32, dev, n)
-    p.weights = _vec(weights, "weights", f32, dev, n)
+    op, rp = _vec(old_logp, "old_logp", f32, dev, n), _vec(ref_logp, "ref_logp", f32, dev, n)
+    ap, wp = _vec(advantages, "advantages", f32, dev, n), _vec(weights, "weights", f32, dev, n)
+    if ap is None:
+        raise ValueError("advantages must be given")
     if not (0 <= clip_low <= 1 and clip_high >= 0 and kl_coef >= 0):
         raise ValueError("clip_low must be in [0, 1], clip_high and kl_coef >= 0")
-    if kl_coef > 0 and ref_logp is None:
+    if kl_coef > 0 and rp is None:
         raise ValueError("kl_coef needs ref_logp")
     if dlogits is not None and not grad:
         raise ValueError("dlogits is given, but grad is False")
@@ -743,13 +766,11 @@ def policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logp: torch.Tensor 
         loss = torch.empty(n, dtype=f32, device=dev)
     if logp is None:
         logp = torch.empty(n, dtype=f32, device=dev)
-    p.loss, p.logp = _vec(loss, "loss", f32, dev, n), _vec(logp, "logp", f32, dev, n)
     if grad:
         dlogits = _grad_out(dlogits, logits, dev, n, V, "dlogits")
-        p.dlogits, p.ld_dlogits = dlogits.data_ptr(), _ld(dlogits)
-    p.logits, p.dtype, p.N, p.V, p.ld = logits.data_ptr(), _DT[logits.dtype], n, V, _ld(logits)
-    p.temperature, p.clip_low, p.clip_high, p.kl_coef = temperature, clip_low, clip_high, kl_coef
-    p.status = _status(status, dev)
+    p = N.PolicyParams(logits.data_ptr(), _DT[logits.dtype], n, V, 0, _ld(logits), ip, op, rp, ap, wp, temperature,
+                       clip_low, clip_high, kl_coef, _vec(loss, "loss", f32, dev, n), _vec(logp, "logp", f32, dev, n),
+                       None, dlogits.data_ptr() if grad else None, _ld(dlogits) if grad else 0, _status(status, dev))
     if n:
         _call(dev, "mstar_policy_loss", ctypes.byref(p))
     return loss, logp, dlogits
