@@ -75,14 +75,20 @@ template <int N>
 struct Roles {
   static constexpr int LANES = N > 32 ? 1 : 2;
   static constexpr int EXPAND = 8 * LANES;                       // expander warps: 32 rows of the tile each
-  static constexpr int SUM = 8;                                  // accumulator warps: the same
+  // Accumulator warps: 32 rows of the tile each, and with 64 columns half of
+  // them: the accumulator is then free for the next MMAs sooner.
+  static constexpr int HALVES = N == 64 ? 2 : 1;
+  static constexpr int SUM = 8 * HALVES;
   static constexpr int ISSUE = 2 * LANES;                        // a warp per half of the tile
-  static constexpr int REST = 8;  // 2 producers, the issuers, the counting warp, in whole warpgroups
+  // Producers and issuers in whole warpgroups; a warp to spare counts the parts
+  // of shared tiles, otherwise the hidden rows' producer does when it is done.
+  static constexpr int REST = (2 + ISSUE + 3) / 4 * 4;
+  static constexpr int COUNTER = REST > 2 + ISSUE ? 2 + ISSUE : 1;
   static constexpr int THREADS = 32 * (EXPAND + SUM + REST);
   static constexpr int LAUNCH = 65536 / THREADS / 8 * 8;
-  static constexpr int REGS_EXPAND = N > 64 ? 48 : N > 32 ? 72 : 64;
-  static constexpr int REGS_SUM = N > 64 ? 160 : N > 32 ? 120 : 80;
-  static constexpr int REGS_REST = N > 64 ? 32 : 48;
+  static constexpr int REGS_EXPAND = N > 64 ? 56 : N > 32 ? 72 : 64;
+  static constexpr int REGS_SUM = N > 64 ? 160 : N > 32 ? 72 : 80;
+  static constexpr int REGS_REST = N > 32 && N <= 64 ? 64 : 48;
   static_assert(32 * (EXPAND * REGS_EXPAND + SUM * REGS_SUM + REST * REGS_REST) <= THREADS * LAUNCH,
                 "registers of the launch");
   // Tensor memory: A buffers [2 blocks][2 tiles][64 columns], then the
@@ -220,8 +226,14 @@ struct Ring {
 // Named barriers 1 and 2 tell the counting warp that a part of this CTA's two
 // shared tiles is written (the accumulator warps arrive and go on); barrier 3
 // tells them what it counted.
-__device__ __forceinline__ void bar_arrive(int id) { asm volatile("bar.arrive %0, 288;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ void bar_sync(int id) { asm volatile("bar.sync %0, 288;" ::"r"(id) : "memory"); }
+template <int N>
+__device__ __forceinline__ void bar_arrive(int id) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(32 * Roles<N>::SUM + 32) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bar_sync(int id) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(32 * Roles<N>::SUM + 32) : "memory");
+}
 
 // KN / 16 MMAs along the columns of one group: A advances by eight columns of
 // tensor memory, B by 32 bytes of its rows, four steps to a box.  Issued by
@@ -584,10 +596,11 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
   using R = Roles<N>;
   constexpr int RING = R::RING;
   constexpr bool MERGED = R::template merged<GPB>();
+  constexpr int NC = N / R::HALVES;       // this warp's columns, from `from`
   constexpr int LC = N == 32 ? 32 : 16;  // columns loaded at a time
   const int warp = (int)(threadIdx.x >> 5) - R::EXPAND, lane = threadIdx.x & 31;
-  const int t = warp >> 2, quad = warp & 3, row = t * 128 + quad * 32 + lane;
-  const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + R::D_COL + (uint32_t)(t * N);
+  const int t = (warp >> 2) & 1, quad = warp & 3, row = t * 128 + quad * 32 + lane, from = (warp >> 3) * NC;
+  const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + R::D_COL + (uint32_t)(t * N + from);
   const bool f32 = g.scale_dtype == MSTAR_DTYPE_F32;
   const bool lane0 = lane == 0;
   const uint32_t full = smem_u32(MERGED ? sh.done[t] : sh.dfull[t]);
@@ -600,9 +613,9 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
   while (w.next(g)) {
     const int v = w.tile / g.nchunks * BM + row, chunk = w.tile % g.nchunks;
     const int64_t s0 = (int64_t)min(v, g.V - 1) * g.ngroups;
-    float acc[N], s[2][GPB];
+    float acc[NC], s[2][GPB];
 #pragma unroll
-    for (int c = 0; c < N; ++c) acc[c] = 0.f;
+    for (int c = 0; c < NC; ++c) acc[c] = 0.f;
     auto fetch = [&](int j, int b) {  // (clamped: groups past the end are never used)
 #pragma unroll
       for (int i = 0; i < GPB; ++i) {
@@ -629,7 +642,7 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
           tc_fence_after();
           const uint32_t at = at0 + (R::SLOTS == 1 ? 0u : (uint32_t)q * 2u * N);
 #pragma unroll
-          for (int c0 = 0; c0 < N; c0 += LC) {
+          for (int c0 = 0; c0 < NC; c0 += LC) {
             uint32_t r[LC / 16][16];
 #pragma unroll
             for (int c = 0; c < LC / 16; ++c) tmem_ld16(at + (uint32_t)(c0 + 16 * c), r[c]);
@@ -648,20 +661,20 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
     if (late) raise(g, sh);
     if (w.k0 == 0 && w.k1 == g.nks) {
 #pragma unroll
-      for (int c0 = 0; c0 < N; c0 += 16)
-        if (!late) put16(g, v, chunk, c0, acc + c0);
+      for (int c0 = 0; c0 < NC; c0 += 16)
+        if (!late) put16(g, v, chunk, from + c0, acc + c0);
       continue;
     }
     // a shared tile: leave the part (the counting warp sees an error by itself)
     const int which = w.k0 == 0 ? 1 : 0, cols = min(g.rows, g.B - chunk * g.rows);
     float *part = g.parts + ((size_t)blockIdx.x * 2 + which) * (size_t)g.n * BM + row;
 #pragma unroll
-    for (int c = 0; c < N; ++c)
-      if (c < cols) __stcg(part + c * BM, acc[c]);
-    bar_arrive(1 + which);
+    for (int c = 0; c < NC; ++c)
+      if (from + c < cols) __stcg(part + (from + c) * BM, acc[c]);
+    bar_arrive<N>(1 + which);
   }
   // the shared tiles for which this CTA's part was the last: add the parts in the order of the columns
-  bar_sync(3);
+  bar_sync<N>(3);
   Work again(g);
   while (again.next(g)) {
     const int which = again.k0 == 0 ? 1 : 0;
@@ -672,7 +685,7 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
     sharers(g, again.tile, c_lo, c_hi);
     const int chunk = again.tile % g.nchunks, cols = min(g.rows, g.B - chunk * g.rows);
 #pragma unroll 1
-    for (int c0 = 0; c0 < cols; c0 += 16) {
+    for (int c0 = from; c0 < min(cols, from + NC); c0 += 16) {
       float sum[16] = {};
       for (int q = c_lo; q < c_hi; ++q) {
         const float *p = g.parts + ((size_t)q * 2 + (unit_start(g, q) <= first ? 1 : 0)) * (size_t)g.n * BM + row;
@@ -688,12 +701,13 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
 }
 
 // Counts the parts of the shared tiles as they are written.
+template <int N>
 __device__ void count_parts(const Gemm &g, Sh &sh, int lane) {
   Work w(g);
   while (w.next(g)) {
     if (w.k0 == 0 && w.k1 == g.nks) continue;
     const int which = w.k0 == 0 ? 1 : 0;
-    bar_sync(1 + which);
+    bar_sync<N>(1 + which);
     if (lane == 0) {
       int c_lo, c_hi;
       sharers(g, w.tile, c_lo, c_hi);
@@ -703,7 +717,7 @@ __device__ void count_parts(const Gemm &g, Sh &sh, int lane) {
     }
     __syncwarp();
   }
-  bar_arrive(3);
+  bar_arrive<N>(3);
 }
 
 template <int N, int GPB>
@@ -728,12 +742,12 @@ __global__ void __launch_bounds__(Roles<N>::THREADS, 1)
     }
     for (int t = 0; t < 2; ++t) {
       for (int j = 0; j < 2; ++j) {
-        mbar_init(&sh.ready[t][j], 4 + (R::template merged<GPB>() ? 4 : 0));
+        mbar_init(&sh.ready[t][j], 4 + (R::template merged<GPB>() ? R::SUM / 2 : 0));
         mbar_init(&sh.done[t][j], 1);
       }
       for (int j = 0; j < 4; ++j) {
         mbar_init(&sh.dfull[t][j], 1);
-        mbar_init(&sh.dempty[t][j], 4);
+        mbar_init(&sh.dempty[t][j], R::SUM / 2);
       }
     }
     for (int j = 0; j < 4; ++j) mbar_init(&sh.mma_done[j], 1);
@@ -768,9 +782,11 @@ __global__ void __launch_bounds__(Roles<N>::THREADS, 1)
       if (lane == 0) produce_hidden(g, sh, sH, &th);
     } else if (warp < FIRST + 2 + R::ISSUE) {
       issue<N, GPB>(g, sh, sH, tbase, warp - FIRST - 2);
-    } else if (warp == FIRST + 2 + R::ISSUE) {
+    }
+    if (warp == FIRST + R::COUNTER) {
+      __syncwarp();
       asm volatile("griddepcontrol.wait;" ::: "memory");
-      count_parts(g, sh, lane);
+      count_parts<N>(g, sh, lane);
     }
   }
   tc_fence_before();
@@ -796,7 +812,7 @@ static Gemm plan(int B, int V, int d) {
   g.nblk = (d + KB - 1) / KB;
   g.ntt = (V + BM - 1) / BM * g.nchunks;
   // (64 rows, V=151936, d=2048: 83 us with three hidden stages, 77 with four)
-  g.hstages = g.n <= 16 ? 8 : g.n <= 32 ? 6 : g.n <= 64 ? 5 : 3;
+  g.hstages = g.n <= 16 ? 8 : g.n <= 32 ? 6 : g.n <= 64 ? 4 : 3;
   g.wstages = std::min(MAX_WS, (SMEM_BUDGET - g.hstages * g.n * KB * 2) / W_BYTES);
   return g;
 }
