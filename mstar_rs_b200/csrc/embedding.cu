@@ -10,7 +10,11 @@
 //
 // Gradient: the tokens are sorted by id first, so each row of the table is
 // summed by one owner in position order (no atomics on values: the same
-// inputs give the same bits) and every row of the output is written once.
+// inputs give the same bits).
+//   fill   the whole output: zeros, or the base.  It is most of the bytes where
+//          the table is large, takes no heed of rows (an odd width would leave
+//          them unaligned) and runs beside the sort; the rows that have tokens
+//          are written over it.
 //   sort   CTA c of C (a power of two) takes the ids v with v mod C = c, which
 //          spreads frequent neighbours, and reads all ids twice: once to count
 //          (per id and per warp, each warp owning a contiguous part of the
@@ -20,8 +24,7 @@
 //          tokens lie together, in position order.
 //   sums   the sorted positions in chunks of equal length, whatever the ids'
 //          frequencies; a chunk writes the runs that start in it, and long runs
-//          that cross its borders leave 32-bit partial sums.  Further CTAs of the same launch
-//          write the rows that no token has.
+//          that cross its borders leave 32-bit partial sums.
 //   joins  the parts of each long run that crosses borders are added in order.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -64,6 +67,20 @@ __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&x)[W]) {
     x[1] = __uint_as_float(u & 0xFFFF0000u);
   } else {
     x[0] = __bfloat162float(p[0]);
+  }
+}
+// 16 bytes as four floats or eight bf16.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4 &w, float *x) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      x[i] = __uint_as_float(u[i]);
+    } else {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
   }
 }
 template <int W>
@@ -116,11 +133,44 @@ __device__ __forceinline__ void bad_id(const Lookup &a, int64_t id, int col) {
   if (id >= a.V && col == 0 && a.status) atomicOr(a.status, MSTAR_STATUS_BAD_ID);
 }
 
+// i / per: a 64-bit division is some seventy instructions, and most lookups have
+// fewer than 2^32 places.
+__device__ __forceinline__ int64_t row_of(int64_t i, uint32_t per, bool small) {
+  return small ? (int64_t)((uint32_t)i / per) : i / per;
+}
+
+// Rows that 16-byte accesses do not fit (an odd width, an unaligned view): a
+// block per row, W values per access.
+template <typename TI, typename TO, int W>
+__global__ void __launch_bounds__(NT) embed_rows_kernel(const Lookup a) {
+  constexpr int U = 4;
+  const int64_t n = blockIdx.x;
+  const int64_t id = a.ids[n];
+  const bool ok = id >= 0 && id < a.V;
+  if (threadIdx.x == 0) bad_id(a, id, 0);
+  const TI *from = static_cast<const TI *>(a.table) + (ok ? id : 0) * a.ld;
+  TO *to = static_cast<TO *>(a.out) + n * a.d;
+  for (int col = (int)threadIdx.x * W; col < a.d; col += NT * W * U) {
+    float x[U][W] = {};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (ok && col + u * NT * W < a.d) load<W>(from + col + u * NT * W, x[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (col + u * NT * W >= a.d) break;
+#pragma unroll
+      for (int j = 0; j < W; ++j) x[u][j] *= a.scale;
+      store<W>(to + col + u * NT * W, x[u]);
+    }
+  }
+}
+
 template <typename TI, typename TO, int W>
 __global__ void __launch_bounds__(NT) embed_kernel(const Lookup a) {
   constexpr int U = 4;
   const uint32_t per = (uint32_t)(a.d / W);
   const int64_t total = a.N * (int64_t)per;
+  const bool small = total <= 0xFFFFFFFFll;
   const int64_t i0 = (int64_t)blockIdx.x * (NT * U) + threadIdx.x;
   float x[U][W];
   int64_t at[U];
@@ -129,7 +179,7 @@ __global__ void __launch_bounds__(NT) embed_kernel(const Lookup a) {
     const int64_t i = i0 + u * NT;
     at[u] = -1;
     if (i >= total) continue;
-    const int64_t n = i / per;
+    const int64_t n = row_of(i, per, small);
     const int col = (int)(i - n * per) * W;
     const int64_t id = a.ids[n];
     at[u] = n * a.d + col;
@@ -156,6 +206,7 @@ __global__ void __launch_bounds__(NT) embed_w4_kernel(const Lookup a) {
   constexpr int U = 4;
   const uint32_t per = (uint32_t)a.d / 8;
   const int64_t total = a.N * (int64_t)per;
+  const bool small = total <= 0xFFFFFFFFll;
   const int64_t i0 = (int64_t)blockIdx.x * (NT * U) + threadIdx.x;
   uint32_t w[U];
   float s[U], z[U];
@@ -165,7 +216,7 @@ __global__ void __launch_bounds__(NT) embed_w4_kernel(const Lookup a) {
     const int64_t i = i0 + u * NT;
     at[u] = -1;
     if (i >= total) continue;
-    const int64_t n = i / per;
+    const int64_t n = row_of(i, per, small);
     const int col = (int)(i - n * per) * 8;
     const int64_t id = a.ids[n];
     at[u] = n * a.d + col;
@@ -194,13 +245,13 @@ __global__ void __launch_bounds__(NT) embed_w4_kernel(const Lookup a) {
 
 constexpr int SORT_NT = 1024;
 constexpr int SORT_NW = SORT_NT / 32;
-constexpr int SORT_U = 16;       // ids per lane and step
+constexpr int SORT_U = 8;        // ids per lane and step
 constexpr int MAX_BINS = SORT_NT;  // ids per CTA of the sort
 constexpr int SUM_NT = 128;
 constexpr int JOIN_G = 8;
 constexpr int MAX_CHUNK = 128;
+constexpr int STAGE_BYTES = 32 * 1024;
 constexpr int LONG_RUN = 32;  // a run of at most this many tokens belongs to the chunk in which it starts
-constexpr int ZERO_ROWS = 32;
 
 struct Grad {
   const void *dout;
@@ -219,12 +270,40 @@ struct Grad {
   float *part;       // [nchunks][2][d]: a run from the chunk before / into the chunk after
 };
 
+// out = base, or zeros, as 16-byte vectors between single bytes.
+constexpr int FILL_NT = 256, FILL_U = 4;
+__global__ void __launch_bounds__(FILL_NT) fill_kernel(uint8_t *out, const uint8_t *base, int64_t bytes) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t stride = (int64_t)gridDim.x * FILL_NT, me = (int64_t)blockIdx.x * FILL_NT + threadIdx.x;
+  const int64_t head = min(bytes, (int64_t)(-reinterpret_cast<intptr_t>(out) & 15));
+  const bool vec = !base || ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(base)) & 15u) == 0;
+  const int64_t nv = vec ? (bytes - head) / 16 : 0;
+  uint4 *o = reinterpret_cast<uint4 *>(out + head);
+  const uint4 *b = base ? reinterpret_cast<const uint4 *>(base + head) : nullptr;
+  int64_t i = me;
+  for (; i + (FILL_U - 1) * stride < nv; i += FILL_U * stride) {
+    uint4 w[FILL_U];
+#pragma unroll
+    for (int u = 0; u < FILL_U; ++u) w[u] = b ? __ldcs(b + i + u * stride) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int u = 0; u < FILL_U; ++u) __stcs(o + i + u * stride, w[u]);
+  }
+  for (; i < nv; i += stride) __stcs(o + i, b ? __ldcs(b + i) : make_uint4(0u, 0u, 0u, 0u));
+  // what the vectors leave: pairs of bytes (both types are of two or four)
+  const int64_t rest = bytes - nv * 16;
+  for (i = me * 2; i < rest; i += stride * 2) {
+    const int64_t at = i < head ? i : i + nv * 16;
+    *reinterpret_cast<uint16_t *>(out + at) = base ? *reinterpret_cast<const uint16_t *>(base + at) : (uint16_t)0;
+  }
+}
+
 // An id's place in the sort's order.
 __device__ __forceinline__ int rank_of(const Grad &a, int v) {
   return (v & ((1 << a.c_log2) - 1)) * a.bins + (v >> a.c_log2);
 }
 
-__global__ void __launch_bounds__(SORT_NT) sort_tokens_kernel(const Grad a) {
+// (40 registers: the fill's blocks keep their place on the SM beside a block of this)
+__global__ void __maxnreg__(40) sort_tokens_kernel(const Grad a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(16) int32_t cnt[];  // [SORT_NW][bins]
   __shared__ int32_t below_w[SORT_NW], scan_w[SORT_NW];
@@ -311,6 +390,8 @@ __global__ void __launch_bounds__(SORT_NT) sort_tokens_kernel(const Grad a) {
       }
     }
   }
+  // the fill runs beside this; what comes after both waits for this kernel alone
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 template <typename TO, int W>
@@ -332,37 +413,20 @@ template <typename TI, typename TO, int W>
 __global__ void __launch_bounds__(SUM_NT) sum_tokens_kernel(const Grad a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int work = a.nchunks * a.col_tiles;
   __shared__ int32_t skey[MAX_CHUNK + LONG_RUN + 2], spos[MAX_CHUNK + LONG_RUN];
-  if ((int)blockIdx.x >= work) {  // rows without a token: zeros, or the base's own
-    const int r0 = ((int)blockIdx.x - work) * ZERO_ROWS, rows = min(ZERO_ROWS, a.V - r0);
-    if ((int)threadIdx.x < rows) {
-      const int k = rank_of(a, r0 + (int)threadIdx.x);
-      skey[threadIdx.x] = a.start[k + 1] - a.start[k];
-    }
-    __syncthreads();
-    for (int r = 0; r < rows; ++r) {
-      if (skey[r]) continue;
-      for (int col = (int)threadIdx.x * W; col < a.d; col += SUM_NT * W) {
-        float acc[W] = {}, b[W];
-        load_base<TO, W>(a, r0 + r, col, b);
-        finish<TO, W>(a, r0 + r, col, acc, b);
-      }
-    }
-    return;
-  }
   const int c = (int)blockIdx.x / a.col_tiles;
   const int col = (((int)blockIdx.x % a.col_tiles) * SUM_NT + (int)threadIdx.x) * W;
-  const int total = a.start[a.bins << a.c_log2];
-  const int s0 = c * a.chunk, s1 = min(total, s0 + a.chunk);
-  if (s0 >= s1) return;
+  const int s0 = c * a.chunk, most = min(a.N, s0 + a.chunk + LONG_RUN) - s0;  // tokens that may be this chunk's
+  const int total = a.start[a.bins << a.c_log2];  // (places past it hold nothing; they are masked below)
   // the chunk's ids and positions first, so that the rows' loads wait for nothing
-  const int seen = min(total, s1 + LONG_RUN) - s0;  // tokens that may be this chunk's
-  for (int i = (int)threadIdx.x; i < seen + 2; i += SUM_NT) {
+  for (int i = (int)threadIdx.x; i < most + 2; i += SUM_NT) {
     const int s = s0 - 1 + i;
-    skey[i] = s >= 0 && s < total ? a.key[s] : -1;
-    if (i < seen) spos[i] = a.pos[s0 + i];
+    const int key = s >= 0 && s < a.N ? a.key[s] : -1, pos = i < most ? a.pos[s0 + i] : 0;
+    skey[i] = s < total ? key : -1;
+    if (i < most) spos[i] = pos;
   }
+  const int s1 = min(total, s0 + a.chunk);
+  if (s0 >= s1) return;
   __syncthreads();
   bool from_before = skey[0] == skey[1];
   int begin = 0, end = s1 - s0;
@@ -376,22 +440,39 @@ __global__ void __launch_bounds__(SUM_NT) sum_tokens_kernel(const Grad a) {
     if (stop - a.start[r] <= LONG_RUN) end = stop - s0;
   }
   if (col >= a.d) return;
-  constexpr int U = 4;
+  // A batch of rows is in flight at once: with 16-byte accesses through
+  // asynchronous copies into shared memory (each thread reads back only what
+  // it copied itself), otherwise through registers.
+  constexpr int BATCH = W == 8 ? STAGE_BYTES / (SUM_NT * W * (int)sizeof(TI)) : 8;
+  constexpr int PARTS = W * (int)sizeof(TI) / 16;  // 16-byte copies per thread and row
+  __shared__ __align__(16) uint8_t stage[W == 8 ? STAGE_BYTES : 16];
   float acc[W] = {}, b[W];
   load_base<TO, W>(a, skey[begin + 1], col, b);  // (read as a run begins: it is there when the run ends)
-  for (int s = begin; s < end; s += U) {
-    float x[U][W];
+  for (int s = begin; s < end; s += BATCH) {
+    const int n = min(BATCH, end - s);
+    float x[W == 8 ? 1 : BATCH][W];
+    if constexpr (W == 8) {
+      for (int u = 0; u < n; ++u) {
+        const TI *from = static_cast<const TI *>(a.dout) + (int64_t)spos[s + u] * a.ldo + col;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s + u < end) load<W>(static_cast<const TI *>(a.dout) + (int64_t)spos[s + u] * a.ldo + col, x[u]);
+        for (int i = 0; i < PARTS; ++i)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                           smem_u32(stage + ((u * PARTS + i) * SUM_NT + (int)threadIdx.x) * 16)),
+                       "l"(reinterpret_cast<const uint4 *>(from) + i)
+                       : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (s + u >= end) break;
+      for (int u = 0; u < BATCH; ++u)
+        if (u < n) load<W>(static_cast<const TI *>(a.dout) + (int64_t)spos[s + u] * a.ldo + col, x[u]);
+    }
+    auto take = [&](int u, const float *y) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) acc[j] += x[u][j];
+      for (int j = 0; j < W; ++j) acc[j] += y[j];
       const int key = skey[s + u + 1];
       const bool goes_on = skey[s + u + 2] == key;
-      if (goes_on && s + u + 1 < end) continue;
+      if (goes_on && s + u + 1 < end) return;
       if (from_before || goes_on) {  // the run crosses a border of the chunk
         store<W>(a.part + ((int64_t)c * 2 + (from_before ? 0 : 1)) * a.d + col, acc);
       } else {
@@ -401,6 +482,21 @@ __global__ void __launch_bounds__(SUM_NT) sum_tokens_kernel(const Grad a) {
 #pragma unroll
       for (int j = 0; j < W; ++j) acc[j] = 0.f;
       if (s + u + 1 < end) load_base<TO, W>(a, skey[s + u + 2], col, b);
+    };
+    if constexpr (W == 8) {
+      for (int u = 0; u < n; ++u) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          const uint4 w = *reinterpret_cast<const uint4 *>(stage + ((u * PARTS + i) * SUM_NT + (int)threadIdx.x) * 16);
+          unpack16<TI>(w, y + i * (8 / PARTS));
+        }
+        take(u, y);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u)
+        if (u < n) take(u, x[u]);
     }
   }
 }
@@ -494,13 +590,12 @@ static int check_lookup(const int64_t *ids, int64_t N, int V, int d, const void 
 
 template <typename TI, typename TO>
 static int launch_lookup(const Lookup &a, int w, cudaStream_t st) {
-  const unsigned grid = (unsigned)((a.N * (a.d / w) + NT * 4 - 1) / (NT * 4));
   if (w == 8)
-    embed_kernel<TI, TO, 8><<<grid, NT, 0, st>>>(a);
+    embed_kernel<TI, TO, 8><<<(unsigned)((a.N * (a.d / 8) + NT * 4 - 1) / (NT * 4)), NT, 0, st>>>(a);
   else if (w == 2)
-    embed_kernel<TI, TO, 2><<<grid, NT, 0, st>>>(a);
+    embed_rows_kernel<TI, TO, 2><<<(unsigned)a.N, NT, 0, st>>>(a);
   else
-    embed_kernel<TI, TO, 1><<<grid, NT, 0, st>>>(a);
+    embed_rows_kernel<TI, TO, 1><<<(unsigned)a.N, NT, 0, st>>>(a);
   return launched();
 }
 
@@ -523,7 +618,7 @@ static Layout layout(int N, int V, int d) {
   Layout l{};
   // chunks long enough to amortise a border, short enough for some waves of CTAs
   const int64_t tiles = (d + SUM_NT * 8 - 1) / (SUM_NT * 8);
-  l.chunk = (int)std::min<int64_t>(MAX_CHUNK, std::max<int64_t>(16, (int64_t)N * tiles / (148 * 16)));
+  l.chunk = (int)std::min<int64_t>(MAX_CHUNK, std::max<int64_t>(32, (int64_t)N * tiles / (148 * 16)));
   l.nchunks = (N + l.chunk - 1) / l.chunk;
   const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
   l.start = 0;
@@ -540,21 +635,34 @@ static int launch_grad(Grad &a, cudaStream_t st) {
   const int smem = SORT_NW * a.bins * 4;
   int rc = allow_smem<sort_tokens_kernel>(smem);
   if (rc) return rc;
-  sort_tokens_kernel<<<1 << a.c_log2, SORT_NT, smem, st>>>(a);
-  if ((rc = launched())) return rc;
-  const int64_t work = (int64_t)a.nchunks * a.col_tiles;
-  const int nzero = a.base == a.out ? 0 : (a.V + ZERO_ROWS - 1) / ZERO_ROWS;
-  // the next kernels may be placed while the one before ends; they wait for it before they read
+  const bool fill = a.base != a.out;
+  if (fill) {  // (two blocks per SM leave the sort its place beside them)
+    const int64_t bytes = (int64_t)a.V * a.d * (int)sizeof(TO);
+    const int64_t blocks = (bytes / 16 + FILL_NT * FILL_U - 1) / (FILL_NT * FILL_U);
+    fill_kernel<<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks, 2 * sm_count())), FILL_NT, 0, st>>>(
+        static_cast<uint8_t *>(a.out), static_cast<const uint8_t *>(a.base), bytes);
+    if ((rc = launched())) return rc;
+  }
+  // the next kernels may be placed while the one before runs; they wait for it before they read
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(work + nzero), 1, 1);
-  cfg.blockDim = dim3(SUM_NT, 1, 1);
+  cfg.gridDim = dim3(1u << a.c_log2, 1, 1);
+  cfg.blockDim = dim3(SORT_NT, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
+  cfg.numAttrs = fill ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, sort_tokens_kernel, a);
+  const int64_t work = (int64_t)a.nchunks * a.col_tiles;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, sum_tokens_kernel<TI, TO, W>, a);
+  cfg.dynamicSmemBytes = 0;
+  if (e == cudaSuccess) {
+    cfg.gridDim = dim3((unsigned)work, 1, 1);
+    cfg.blockDim = dim3(SUM_NT, 1, 1);
+    e = cudaLaunchKernelEx(&cfg, sum_tokens_kernel<TI, TO, W>, a);
+  }
   if (e == cudaSuccess && a.nchunks > 1) {
     cfg.gridDim = dim3((unsigned)std::min(a.nchunks - 1, 148), (unsigned)a.col_tiles, 1);
     cfg.blockDim = dim3(SUM_NT * JOIN_G, 1, 1);

@@ -86,9 +86,9 @@ struct Roles {
   static constexpr int COUNTER = REST > 2 + ISSUE ? 2 + ISSUE : 1;
   static constexpr int THREADS = 32 * (EXPAND + SUM + REST);
   static constexpr int LAUNCH = 65536 / THREADS / 8 * 8;
-  static constexpr int REGS_EXPAND = N > 64 ? 56 : N > 32 ? 72 : 64;
-  static constexpr int REGS_SUM = N > 64 ? 160 : N > 32 ? 72 : 80;
-  static constexpr int REGS_REST = N > 32 && N <= 64 ? 64 : 48;
+  static constexpr int REGS_EXPAND = N > 64 ? 56 : 64;
+  static constexpr int REGS_SUM = N > 64 ? 160 : 80;
+  static constexpr int REGS_REST = 48;
   static_assert(32 * (EXPAND * REGS_EXPAND + SUM * REGS_SUM + REST * REGS_REST) <= THREADS * LAUNCH,
                 "registers of the launch");
   // Tensor memory: A buffers [2 blocks][2 tiles][64 columns], then the
@@ -597,7 +597,7 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
   constexpr int RING = R::RING;
   constexpr bool MERGED = R::template merged<GPB>();
   constexpr int NC = N / R::HALVES;       // this warp's columns, from `from`
-  constexpr int LC = N == 32 ? 32 : 16;  // columns loaded at a time
+  constexpr int LC = N == 32 || N == 64 ? 32 : 16;  // columns loaded at a time
   const int warp = (int)(threadIdx.x >> 5) - R::EXPAND, lane = threadIdx.x & 31;
   const int t = (warp >> 2) & 1, quad = warp & 3, row = t * 128 + quad * 32 + lane, from = (warp >> 3) * NC;
   const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + R::D_COL + (uint32_t)(t * N + from);
@@ -647,13 +647,17 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
 #pragma unroll
             for (int c = 0; c < LC / 16; ++c) tmem_ld16(at + (uint32_t)(c0 + 16 * c), r[c]);
             tmem_wait_ld();
+            if (c0 + LC == NC) {  // all is in registers: the accumulator is free
+              tc_fence_before();
+              // (with one lane it is the next block's, otherwise this lane's next)
+              arrive(!MERGED ? dempty + 8u * q
+                             : ready + 8u * (R::LANES == 2 ? j : j == 0 && b + 1 < g.nblk ? 1 : 0),
+                     lane0);
+            }
 #pragma unroll
             for (int c = 0; c < LC; c += 2)
               fma2(acc[c0 + c], acc[c0 + c + 1], r[c / 16][c % 16], r[c / 16][c % 16 + 1], s[j][gi]);
           }
-          tc_fence_before();
-          // (with one lane the accumulator is the next block's, otherwise this lane's next)
-          arrive(!MERGED ? dempty + 8u * q : ready + 8u * (R::LANES == 2 ? j : j == 0 && b + 1 < g.nblk ? 1 : 0), lane0);
         }
         fetch(j, b + 2);
       }
@@ -684,18 +688,21 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
     int c_lo, c_hi;
     sharers(g, again.tile, c_lo, c_hi);
     const int chunk = again.tile % g.nchunks, cols = min(g.rows, g.B - chunk * g.rows);
+    constexpr int JC = NC < 128 ? 16 : 32;  // columns at a time
 #pragma unroll 1
-    for (int c0 = from; c0 < min(cols, from + NC); c0 += 16) {
-      float sum[16] = {};
+    for (int c0 = from; c0 < min(cols, from + NC); c0 += JC) {
+      float sum[JC] = {};
       for (int q = c_lo; q < c_hi; ++q) {
         const float *p = g.parts + ((size_t)q * 2 + (unit_start(g, q) <= first ? 1 : 0)) * (size_t)g.n * BM + row;
-        float x[16];  // (columns past the last read it again: no load waits for another)
+        float x[JC];  // (columns past the last read it again: no load waits for another)
 #pragma unroll
-        for (int c = 0; c < 16; ++c) x[c] = __ldcg(p + min(c0 + c, cols - 1) * BM);
+        for (int c = 0; c < JC; ++c) x[c] = __ldcg(p + min(c0 + c, cols - 1) * BM);
 #pragma unroll
-        for (int c = 0; c < 16; ++c) sum[c] += x[c];
+        for (int c = 0; c < JC; ++c) sum[c] += x[c];
       }
-      put16(g, v, chunk, c0, sum);
+#pragma unroll
+      for (int c = 0; c < JC; c += 16)
+        if (c0 + c < cols) put16(g, v, chunk, c0 + c, sum + c);
     }
   }
 }
