@@ -368,7 +368,6 @@ def lmhead_step(hidden: torch.Tensor, weight: torch.Tensor, logits: torch.Tensor
 
 # ------------------------------------------------- 4-bit weights, lookup, log-probabilities, policy loss
 
-_ES = {torch.float32: 4, torch.bfloat16: 2}
 _FN: dict = {}  # entry points by name, once the library is loaded
 
 
@@ -441,13 +440,19 @@ def _ld(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
+def _span(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to behind its last."""
+    if t.numel() == 0:
+        return 0
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two matrices' memory ranges meet without being the same rows."""
     if a.data_ptr() == b.data_ptr() and _ld(a) == _ld(b) and a.dtype == b.dtype:
         return False
-    span = lambda t: ((t.shape[0] - 1) * _ld(t) + t.shape[1]) * _ES[t.dtype]  # noqa: E731
     a0, b0 = a.data_ptr(), b.data_ptr()
-    return a0 < b0 + span(b) and b0 < a0 + span(a)
+    return a0 < b0 + _span(b) and b0 < a0 + _span(a)
 
 
 def quantize_w4(weight: torch.Tensor, group_size: int = 128, *, zero_points: bool = False, scale_dtype=torch.bfloat16):
@@ -576,7 +581,7 @@ def _ids_1d(ids, dev):
     return ids.numel()
 
 
-def _lookup_out(ids, d, out, dtype, dev):
+def _lookup_out(ids, d, out, dtype, dev, table):
     if out is None:
         if dtype not in _DT:
             raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
@@ -585,6 +590,9 @@ def _lookup_out(ids, d, out, dtype, dev):
         raise TypeError(f"out must be float32 or bfloat16, got {out.dtype}")
     if out.device != dev or out.shape != (*ids.shape, d) or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {(*ids.shape, d)} tensor on {dev}")
+    a0, b0 = out.data_ptr(), table.data_ptr()
+    if a0 < b0 + _span(table) and b0 < a0 + _span(out):
+        raise ValueError("out must not overlap the table")
     return out
 
 
@@ -601,7 +609,7 @@ def embed_tokens(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, 
     V, d = table.shape
     _matrix(table, "table", dev, V, d)
     n = _ids_1d(ids, dev)
-    out = _lookup_out(ids, d, out, dtype or table.dtype, dev)
+    out = _lookup_out(ids, d, out, dtype or table.dtype, dev, table)
     st = _status(status, dev)
     if n:
         _call(dev, "mstar_embed_tokens", ids.data_ptr(), n, table.data_ptr(), _DT[table.dtype], V, d, _ld(table),
@@ -617,7 +625,7 @@ def embed_tokens_w4(ids: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
     w = _w4(codes, scales, zeros)
     dev = codes.device
     n = _ids_1d(ids, dev)
-    out = _lookup_out(ids, w.d, out, dtype, dev)
+    out = _lookup_out(ids, w.d, out, dtype, dev, codes)
     st = _status(status, dev)
     if n:
         _call(dev, "mstar_embed_tokens_w4", ids.data_ptr(), n, ctypes.byref(w), scale, out.data_ptr(), _DT[out.dtype],
