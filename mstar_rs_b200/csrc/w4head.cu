@@ -10,8 +10,9 @@
 // The operands are fp16 and not bf16 because its ten bits take a code at two
 // places of a word (below), which spares two of seven integer instructions;
 // so each hidden row is first scaled by a power of two that brings its largest
-// value into [2^14, 2^15).  A bf16 value keeps all its bits down to 2^-31 of the
-// row's largest and is off by at most 2^-40 of that below.
+// value into [2^15, 2^16).  A bf16 value keeps all its bits down to 2^-32 of the
+// row's largest; below that it is off by at most half of fp16's smallest step,
+// 2^-25, which is 2^-40 of the largest.
 //
 // With few rows the weight stream bounds the product (V * d / 2 bytes), next
 // to it turning the codes into fp16 (nine instructions for eight weights) and
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(PREP_NT)
   if (top) {
     int x;
     frexpf(__uint_as_float(top << 16), &x);  // the largest is in [2^(x-1), 2^x)
-    e = 15 - x;
+    e = 16 - x;  // at most (2 - 2^-7) 2^15 = 65280, below fp16's largest; 2^-e >= 2^-148 is a float
   }
   if (tid == 0) row_scale[blockIdx.x] = ldexpf(1.f, -e);
   for (int i = tid; i < per; i += PREP_NT) {

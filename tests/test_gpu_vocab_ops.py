@@ -491,3 +491,163 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for k in (0, 1):
         assert all(torch.equal(a, b) for a, b in zip(graphs[k][1], want[k]))
+
+
+# ------------------------------------------------------------ refusals, sizes past 32 bits
+
+
+def test_front_end_refusals():
+    from mstar_rs_b200 import kernel as k
+
+    dev = "cuda"
+    x, ids, f = torch.zeros(4, 64, device=dev), torch.zeros(4, dtype=torch.int64, device=dev), torch.zeros(4, device=dev)
+    codes, scales = torch.zeros(8, 32, dtype=torch.uint8, device=dev), torch.ones(8, 1, device=dev)
+    h = torch.zeros(4, 64, device=dev, dtype=BF16)
+    cases = [
+        (TypeError, lambda: k.token_logprobs(x.half(), ids)), (TypeError, lambda: k.token_logprobs(x, ids.int())),
+        (ValueError, lambda: k.token_logprobs(x[0], ids)), (ValueError, lambda: k.token_logprobs(x, ids[:3])),
+        (ValueError, lambda: k.token_logprobs(x.t(), ids)), (ValueError, lambda: k.token_logprobs(x, ids, temperature=0.0)),
+        (ValueError, lambda: k.token_logprobs(x, ids.cpu())),
+        (ValueError, lambda: k.token_logprobs(x[:1].expand(4, 64), ids)),  # rows on top of one another
+        (ValueError, lambda: k.token_logprobs(x, ids, status=f)),
+        (TypeError, lambda: k.token_logprobs_grad(x, ids, f, f.double())),
+        (TypeError, lambda: k.token_logprobs_grad(x, ids, f, f, out=torch.zeros(4, 64, device=dev, dtype=BF16))),
+        (ValueError, lambda: k.token_logprobs_grad(x[:, :60], ids, f, f, out=x[:, 4:])),  # overlapping, not the same
+        (ValueError, lambda: k.policy_loss(x, ids, f, None)), (ValueError, lambda: k.policy_loss(x, ids, f, f, kl_coef=0.1)),
+        (ValueError, lambda: k.policy_loss(x, ids, f, f, clip_low=2.0)),
+        (ValueError, lambda: k.policy_loss(x, ids, f, f, kl_coef=math.nan, ref_logp=f)),
+        (ValueError, lambda: k.policy_loss(x, ids, f, f, grad=False, dlogits=x)),
+        (ValueError, lambda: k.policy_loss(x, ids, f[:2], f)),
+        (TypeError, lambda: k.embed_tokens(ids, x.half())), (TypeError, lambda: k.embed_tokens(ids, x, dtype=torch.float16)),
+        (ValueError, lambda: k.embed_tokens(ids, x, out=x)), (ValueError, lambda: k.embed_tokens(ids[::2], x)),
+        (ValueError, lambda: k.embed_tokens(ids, x, out=torch.zeros(3, 64, device=dev))),
+        (ValueError, lambda: k.embed_tokens_grad(ids, x[:3], 9)), (ValueError, lambda: k.embed_tokens_grad(ids, x, 0)),
+        (ValueError, lambda: k.embed_tokens_grad(ids, x, 4, out=x)),
+        (TypeError, lambda: k.embed_tokens_grad(ids, x, 4, base=torch.zeros(4, 64, device=dev), dtype=BF16)),
+        (ValueError, lambda: k.embed_tokens_grad(ids, x, 9, base=torch.zeros(4, 64, device=dev))),
+        (ValueError, lambda: k.embed_tokens_w4(ids, codes, scales, zeros=torch.zeros(8, 2, dtype=torch.uint8, device=dev))),
+        (TypeError, lambda: k.embed_tokens_w4(ids, codes, scales.half())),
+        (ValueError, lambda: k.embed_tokens_w4(ids, codes, torch.ones(8, 4, device=dev))),  # groups of 16
+        (TypeError, lambda: k.lmhead_logits_w4(x, codes, scales)), (ValueError, lambda: k.lmhead_logits_w4(h[:, :32], codes, scales)),
+        (ValueError, lambda: k.lmhead_logits_w4(torch.zeros(257, 64, device=dev, dtype=BF16), codes, scales)),
+        (ValueError, lambda: k.lmhead_logits_w4(h, codes, scales, out=torch.zeros(4, 9, device=dev))),
+        (ValueError, lambda: k.lmhead_logits_w4(h, codes, scales, workspace=f)),
+    ]
+    for error, call in cases:
+        with pytest.raises(error):
+            call()
+    torch.cuda.synchronize()
+    assert bool((x == 0).all())
+
+
+def test_nothing_to_do():
+    """No rows: empty results, no launch; the lookup's gradient of no tokens
+    is the base, or zeros."""
+    from mstar_rs_b200 import kernel as k
+
+    x, ids, f = torch.zeros(0, 64, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda"), torch.zeros(0, device="cuda")
+    assert k.token_logprobs(x, ids)[0].shape == (0,)
+    assert k.token_logprobs_grad(x, ids, f, f).shape == (0, 64)
+    assert k.policy_loss(x, ids, f, f)[2].shape == (0, 64)
+    base = torch.randn(5, 64, device="cuda")
+    assert bool((k.embed_tokens_grad(ids, x, 5) == 0).all())
+    assert torch.equal(k.embed_tokens_grad(ids, x, 5, base=base), base)
+    assert k.embed_tokens_grad(ids, x, 5, base=base, out=base) is base
+
+
+def test_places_past_32_bits():
+    """Rows, tables and weights whose last elements lie beyond 2^31 of them."""
+    from mstar_rs_b200 import kernel as k
+
+    V, n = 151936, 14300
+    x = torch.zeros(n, V, device="cuda", dtype=BF16)
+    x[-2:] = torch.randn(2, V, device="cuda", generator=gen(1)).to(BF16)
+    ids = torch.full((n,), V - 1, device="cuda")
+    adv = torch.ones(n, device="cuda")
+    assert (n - 2) * V > 2 ** 31
+    loss, logp, dx = k.policy_loss(x, ids, None, adv, dlogits=None)
+    _, lse, lp = R.rows(x[-2:], ids[-2:], 1.0)
+    near(logp[-2:], lp, R.SUM + lp.abs() * 2.0 ** -23)
+    ref, tol = R.grad(x[-2:], ids[-2:], 1.0, lse, -adv[-2:].double(), BF16)
+    near(dx[-2:], ref, tol)
+    assert abs(float(logp[0]) + math.log(V)) <= R.SUM + 13 * 2.0 ** -23
+    del x, dx, loss
+    V, d = 1_700_000, 1300
+    table = torch.zeros(V, d, device="cuda", dtype=BF16)
+    table[-3:] = torch.randn(3, d, device="cuda", generator=gen(2)).to(BF16)
+    ids = torch.tensor([V - 1, 0, V - 3], device="cuda")
+    assert torch.equal(k.embed_tokens(ids, table), table[ids])
+    del table
+    dout = torch.randn(3, d, device="cuda", generator=gen(3)).to(BF16)
+    g = k.embed_tokens_grad(ids, dout, V)
+    assert torch.equal(g[ids], dout) and not bool(g[1:-3].any()) and not bool(g[-2].any())
+    del g
+    V, d = 1_100_000, 4096
+    codes = torch.full((V, d // 2), 0x88, device="cuda", dtype=torch.uint8)
+    codes[-5:] = torch.randint(0, 256, (5, d // 2), device="cuda", dtype=torch.uint8, generator=gen(4))
+    scales = torch.full((V, d // 128), 0.01, device="cuda")
+    hidden = torch.randn(2, d, device="cuda", generator=gen(5)).to(BF16)
+    out = k.lmhead_logits_w4(hidden, codes, scales)
+    ref, tol = R.head(hidden, codes[-5:], scales[-5:], None, F32, parts=16)
+    near(out[:, -5:], ref, tol)
+    assert not bool(out[:, :-5].any())
+    assert torch.equal(k.embed_tokens_w4(torch.tensor([V - 2], device="cuda"), codes, scales, dtype=F32).double(),
+                       R.dequant(codes[-2:-1], scales[-2:-1], None).float().double())
+
+
+def test_another_stream_than_the_tensors_own():
+    """Inputs made on one stream, the calls on another that waits for it."""
+    from mstar_rs_b200 import kernel as k
+
+    codes, scales, _ = w4_inputs(30000, 512, 64, BF16, False, 1)
+    hidden = torch.randn(7, 512, device="cuda", generator=gen(2)).to(BF16)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        out = k.lmhead_logits_w4(hidden, codes, scales)
+        ids = out.argmax(1)
+        logp, lse = k.token_logprobs(out, ids)
+        g = k.embed_tokens_grad(ids, hidden, 30000, dtype=F32)
+    torch.cuda.current_stream().wait_stream(s)
+    ref, tol = R.head(hidden, codes, scales, None, F32, parts=16)
+    near(out, ref, tol)
+    _, _, lp = R.rows(out, ids, 1.0)
+    near(logp, lp, R.SUM + lp.abs() * 2.0 ** -23)
+    gref, gtol = R.embed_grad(ids, hidden, 30000, 1.0, None, F32)
+    near(g, gref, gtol)
+
+
+def test_infinities_and_nan_in_hidden_rows():
+    """A row's infinity meets codes at their zero point as NaN and others as
+    an infinity, as the products say; other rows keep theirs."""
+    from mstar_rs_b200 import kernel as k
+
+    V, d = 260, 256
+    codes, scales, z = w4_inputs(V, d, 64, F32, True, 8)
+    hidden = torch.randn(4, d, device="cuda", generator=gen(9)).to(BF16)
+    hidden[1, 5], hidden[2, 7], hidden[3] = math.inf, math.nan, 0.0
+    out = k.lmhead_logits_w4(hidden, codes, scales, zeros=z)
+    want = hidden.double() @ R.dequant(codes, scales, z).t()
+    assert torch.equal(out[1].isnan(), want[1].isnan()) and torch.equal(out[1] > 0, want[1] > 0)
+    assert bool(out[1].isfinite().logical_not().all()) and bool(out[2].isnan().all()) and not bool(out[3].any())
+    ref, tol = R.head(hidden[:1], codes, scales, z, F32, parts=16)
+    near(out[:1], ref, tol)
+
+
+def test_small_hidden_values_beside_a_large_one():
+    """Values 2^-31 of the row's largest keep their bits; below that they are
+    off by at most 2^-40 of it."""
+    from mstar_rs_b200 import kernel as k
+
+    V, d = 300, 128
+    codes = torch.full((V, d // 2), 0x99, device="cuda", dtype=torch.uint8)  # every weight 1
+    codes[:, 0] = 0x98  # column 0: weight 0
+    scales = torch.ones(V, 1, device="cuda")
+    for big in (1.0, 2.0 ** 100, 2.0 ** -90):
+        for e in (20, 31, 36):
+            hidden = torch.zeros(1, d, device="cuda")
+            hidden[0, 0], hidden[0, 9] = big, big * 2.0 ** -e * 1.1015625
+            hidden = hidden.to(BF16)
+            out = k.lmhead_logits_w4(hidden, codes, scales)
+            err = (out.double() - hidden[0, 9].double()).abs().max()
+            assert err <= (0.0 if e <= 31 else big * 2.0 ** -40), (big, e, float(err))
