@@ -310,7 +310,8 @@ int mstar_embed_tokens_grad(const int64_t *ids, int32_t N, const void *dout, int
  * lse[n] = log sum_v exp(logits[n, v] / temperature) (or NULL) and logp[n] =
  * logits[n, ids[n]] / temperature - lse[n].  -inf logits are masked ids; a
  * row of nothing else is empty: lse and logp are -inf and *status gets
- * MSTAR_STATUS_EMPTY.  NaN and +inf make their row NaN.  A negative id is a
+ * MSTAR_STATUS_EMPTY (another row's lse is finite: beyond the floats it is
+ * their largest or lowest).  NaN and +inf make their row NaN.  A negative id is a
  * padding row with logp 0; an id >= V counts as one and sets
  * MSTAR_STATUS_BAD_ID.  temperature in [1e-5, 1e5]. */
 int mstar_token_logprobs(const void *logits, int32_t dtype, int32_t N, int32_t V, int64_t ld, const int64_t *ids,
@@ -319,7 +320,11 @@ int mstar_token_logprobs(const void *logits, int32_t dtype, int32_t N, int32_t V
 /* The gradient of sum_n dlogp[n] * logp[n] to the logits: dlogits[n, v] =
  * dlogp[n] / temperature * ([v == ids[n]] - exp(logits[n, v] / temperature -
  * lse[n])), of the logits' type; dlogits may be logits itself (replaced in
- * place), otherwise it must not overlap it.  Padding and empty rows: zeros. */
+ * place), otherwise it must not overlap it.  lse is mstar_token_logprobs', or
+ * that of a longer row of which logits holds a part.  32 bits hold an lse to
+ * 2^-24 of itself: from |lse| = 65536 on (every id of a row under a finite
+ * mask), one that agrees with the row's own to that is replaced by it.
+ * Padding and empty rows (lse -inf): zeros. */
 int mstar_token_logprobs_grad(const void *logits, int32_t dtype, int32_t N, int32_t V, int64_t ld, const int64_t *ids,
                               double temperature, const float *lse, const float *dlogp, void *dlogits,
                               int64_t ld_dlogits, void *stream);

@@ -30,6 +30,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "common.cuh"
@@ -45,9 +46,12 @@ constexpr int MAX_S = 8;                  // portable cluster width
 constexpr int SLICE_BYTES = 80 * 1024;  // of a row per CTA, where there are rows enough
 // Values at or below FLOOR count as masked while the running maximum is
 // tracked (a mask of the type's lowest value would overflow when scaled by
-// c); a row whose largest value is not inside (FLOOR, -FLOOR) takes the
-// exact path, which subtracts before it scales.
+// c).  A row whose scaled maximum M is not inside (-EDGE, EDGE) takes the exact
+// path, which subtracts before it scales: terms carry M's rounding, at most 2^5
+// below EDGE = 2^30, but from 2^32 on it leaves the exponent's range (a row whose
+// every id is masked by -1e10).
 constexpr float FLOOR = -1e30f;
+constexpr float EDGE = 0x1p30f;
 
 enum : int { LOGPROBS = 0, POLICY = 1, POLICY_GRAD = 2 };
 
@@ -278,6 +282,12 @@ struct Token {
   }
 };
 
+// lse as a float: -infinity stands for an empty row, so what 32 bits cannot
+// hold (the lowest value over a T below 1) becomes their largest or lowest.
+__device__ __forceinline__ float finite(double lse) {
+  return fabs(lse) > (double)FLT_MAX ? (float)copysign((double)FLT_MAX, lse) : (float)lse;
+}
+
 // The row's scalars in 64 bits, by a whole warp (its lanes hold the same
 // values; the ratio and the KL term take a lane each): xr is the maximum
 // that the sum s is relative to.  Every CTA of the row computes them; one
@@ -293,7 +303,7 @@ __device__ __forceinline__ Scalars scalars(const Args &a, int row, int64_t id, b
   writer = writer && lane == 0;
   if (writer) {
     a.logp[row] = (float)lp;
-    if (a.lse) a.lse[row] = (float)lse;
+    if (a.lse) a.lse[row] = empty ? -INFINITY : finite(lse);
     const uint32_t bits = (empty ? MSTAR_STATUS_EMPTY : 0u) | (id >= a.V ? MSTAR_STATUS_BAD_ID : 0u);
     if (a.status && bits) atomicOr(a.status, bits);
   }
@@ -423,7 +433,7 @@ __global__ void __launch_bounds__(NT, 6) token_rows_kernel(const Args a) {
   float2 t = cluster_join<0>(sh, S, rank, st.M, st.s0 + st.s1, true);
   if (tid < 32) {
     Scalars r{};
-    const bool exact = !(t.x > FLOOR * c && t.x < -FLOOR * c);
+    const bool exact = !(t.x > -EDGE && t.x < EDGE);
     if (!exact) r = scalars<MODE>(a, row, id, ok, (double)t.x / (double)c, t.y, false, tok, rank == 0);
     r.M = t.x;
     r.exact = exact;
@@ -480,6 +490,42 @@ struct GradArgs {
   int64_t ldd;
 };
 
+// A row whose |lse| is at least FAR (every id under a finite mask, or a tiny T):
+// 32 bits hold such an lse to 2^-8 at best, from 2^24 on not even to log V, so
+// one block sums the row anew.  The sum's own lse counts where the given one is
+// a rounding of it; another (of a row that is part of a longer one) is taken as
+// given.  The first pass ends before the second writes: dlogits may be logits.
+constexpr float FAR = 65536.f;
+
+template <typename T>
+__device__ __noinline__ void far_row_grad(const T *in, T *out, int V, int id, float c, double inv_t, float lse,
+                                          float g) {
+  __shared__ float part[NW];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float m = -INFINITY;
+  for (int v = tid; v < V; v += NT) m = fmaxf(m, to_f(in[v]));
+  m = warp_max(m);
+  if (lane == 0) part[warp] = m;
+  __syncthreads();
+  m = warp_max(part[lane & (NW - 1)]);
+  if (m == -INFINITY) m = 0.f;  // a part of a row that holds masked ids alone: its values give 0
+  float s = 0.f;
+  for (int v = tid; v < V; v += NT) s += ex2((to_f(in[v]) - m) * c);
+  s = warp_sum(s);
+  __syncthreads();
+  if (lane == 0) part[warp] = s;
+  __syncthreads();
+  s = warp_sum(lane < NW ? part[lane] : 0.f);
+  const double own = (double)m * inv_t + log((double)s), given = lse;
+  // -g exp(x / T - lse) = k 2^((x - m) c)
+  const bool same = fabs((double)finite(own) - given) <= fabs(given) * 0x1p-23;
+  const float k = same ? -g / s : (float)(-(double)g * exp((double)m * inv_t - given));
+  for (int v = tid; v < V; v += NT) {
+    const float p = ex2((to_f(in[v]) - m) * c);
+    put(out + v, (p == 0.f ? 0.f : p * k) + (v == id ? g : 0.f));
+  }
+}
+
 // dlogits = dlogp / T * (onehot - 2^(x c - lse T c)): lse enters through its
 // own reference point lse * T, so c's rounding is relative to x - lse * T, and
 // the part of lse T c that 32 bits lose goes into the row's factor.
@@ -488,6 +534,7 @@ __global__ void __launch_bounds__(NT) token_logprobs_grad_kernel(const GradArgs 
   constexpr int E = Vec<T>::E;
   constexpr int U = 4;  // vectors in flight per thread
   __shared__ float sM, sk, sg;
+  __shared__ bool far;
   const int S = a.S, rank = (int)(blockIdx.x % (unsigned)S), row = (int)(blockIdx.x / (unsigned)S);
   const int tid = threadIdx.x;
   const Row<T> in(static_cast<const T *>(a.logits) + (int64_t)row * a.ld, a.V);
@@ -506,8 +553,13 @@ __global__ void __launch_bounds__(NT) token_logprobs_grad_kernel(const GradArgs 
     sM = ok ? (float)M : 0.f;
     sg = g;
     sk = ok ? -g * ex2((float)((double)(float)M - M)) : 0.f;
+    far = ok && fabsf(lse) >= FAR && fabsf(lse) < INFINITY;
   }
   __syncthreads();
+  if (far) {
+    if (rank == 0) far_row_grad<T>(in.p, out, a.V, (int)id, a.c, a.inv_t, a.lse[row], sg);
+    return;
+  }
   const float M = sM, k = sk, g = sg, c = a.c;
   if (fringe >= 0) {
     const float x = to_f(in.p[fringe]);

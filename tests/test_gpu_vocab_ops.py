@@ -651,3 +651,59 @@ def test_small_hidden_values_beside_a_large_one():
             out = k.lmhead_logits_w4(hidden, codes, scales)
             err = (out.double() - hidden[0, 9].double()).abs().max()
             assert err <= (0.0 if e <= 31 else big * 2.0 ** -40), (big, e, float(err))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradient_of_rows_far_from_zero(dtype):
+    """Rows whose lse 32 bits cannot hold to log V: the softmax of the row
+    itself, as the policy loss takes it.  An lse that is not the row's own (a
+    part of a longer row) is taken as given."""
+    from mstar_rs_b200 import kernel as k
+
+    V = 3001
+    low = torch.finfo(dtype).min
+    for T in (1.0, 0.7, 1e-5):
+        x = torch.randn(8, V, device="cuda", generator=gen(3)).to(dtype)
+        x[0], x[1], x[2] = low, -1e10, 1e10
+        x[3], x[3, 7] = -1e9, -math.inf
+        x[4] = x[4] + 70000
+        x[5], x[5, 1:] = 3e38, low
+        x[6] = low
+        x[6, :2] = -1e30
+        ids = torch.tensor([5, 5, 0, 9, 5, 0, 1, 5], device="cuda")
+        dlogp = torch.randn(8, device="cuda", generator=gen(4))
+        logp, lse = k.token_logprobs(x, ids, temperature=T)
+        got = k.token_logprobs_grad(x, ids, lse, dlogp, temperature=T)
+        _, true, lp = R.rows(x, ids, T)
+        near(logp, lp, R.SUM + lp.abs() * 2.0 ** -23)
+        xd = x.double() / T
+        m = xd.amax(1, keepdim=True)
+        p = (xd - m).exp()
+        p = p / p.sum(1, keepdim=True)
+        hot = torch.zeros_like(p)
+        hot[torch.arange(8, device="cuda"), ids] = 1.0
+        g = (dlogp.double() / T)[:, None]
+        ref = g * (hot - p)
+        # the probability: SUM, and 2^-22 of its exponent; row 7 (and every row
+        # with |lse| < 65536) also takes lse's half step, 2^-24 of it
+        arg = torch.where(p > 0, (m - xd).clamp(max=1000) * 1.4427 * 2.0 ** -22, 0.0)
+        half = torch.where(true.abs() < 65536, true.abs() * 2.0 ** -24, 0.0)[:, None]
+        tol = g.abs() * (p * (R.SUM + arg + half) + (hot + p) * 2.0 ** -23) + ref.abs() * R.HALF[dtype] + 2.0 ** -125 * (1 + g.abs())
+        near(got, ref, tol)
+        same = x.clone()
+        assert k.token_logprobs_grad(same, ids, lse, dlogp, temperature=T, out=same) is same and torch.equal(same, got)
+        loss, lp2, dx = k.policy_loss(x, ids, None, -dlogp, temperature=T)  # r = 1: the same gradient
+        assert torch.equal(lp2, logp)
+        near(dx, ref, tol)
+    # half of a row, with the whole row's lse
+    x = (torch.randn(1, 2000, device="cuda", generator=gen(5)) + 2.0 ** 17).float()
+    x[:, 1000:] += 4.0  # (so that the whole row's lse is 4 above the half's: 2^17 has steps of 2^-6)
+    ids = torch.tensor([3], device="cuda")
+    one = torch.ones(1, device="cuda")
+    _, lse = k.token_logprobs(x, ids)
+    got = k.token_logprobs_grad(x[:, :1000], ids, lse, one)
+    ref, tol = R.grad(x[:, :1000], ids, 1.0, lse.double(), one.double(), F32)
+    near(got, ref, tol)
+    x[:, :1000] = -math.inf
+    got = k.token_logprobs_grad(x[:, :1000], ids, lse, one)
+    assert got[0, 3] == 1 and not bool(got[0, :3].any()) and not bool(got[0, 4:].any())
