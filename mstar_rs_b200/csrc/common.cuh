@@ -7,6 +7,7 @@
 
 #include <atomic>
 #include <cstdint>
+#include <mutex>
 #include <string>
 
 #include "../../include/mstar_sampler.h"
@@ -76,17 +77,19 @@ int sm_count();
 int max_smem_optin();
 
 // Lets kernel K use `bytes` of dynamic shared memory on the current device;
-// the runtime is asked once per device and larger size.
+// the runtime is asked once per device and larger size (by one thread at a time:
+// a smaller size set last would undo a larger one).
 template <auto K>
 inline int allow_smem(int bytes) {
   static std::atomic<int> allowed[kMaxDevices];
+  static std::mutex setting;
   std::atomic<int> &have = allowed[current_device()];
+  if (have.load(std::memory_order_acquire) >= bytes) return MSTAR_OK;
+  const std::lock_guard<std::mutex> lock(setting);
   if (have.load(std::memory_order_relaxed) >= bytes) return MSTAR_OK;
   const cudaError_t e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(MSTAR_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
-  int old = have.load(std::memory_order_relaxed);
-  while (old < bytes && !have.compare_exchange_weak(old, bytes)) {
-  }
+  have.store(bytes, std::memory_order_release);
   return MSTAR_OK;
 }
 
