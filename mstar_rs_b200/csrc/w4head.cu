@@ -120,6 +120,7 @@ struct Gemm {
   const void *scales;
   int scale_dtype;
   const uint8_t *zeros;
+  int wide_scales, wide_zeros;  // whether their rows allow wide loads
   void *out;
   int64_t ld;
   int out_dtype;
@@ -501,21 +502,41 @@ __device__ void expand_rows(const Gemm &g, Sh &sh, const uint8_t *sW, uint32_t t
   Ring st;
   uint32_t dp = 0, fresh = 3u;  // parities of done[t][j], a bit each; unused A buffers
   uint32_t nz[GPB], nz16[GPB], late = 0;
+  // zero points: as the scales, eight bytes at a time with groups below 128 (151
+  // against 144 us, 64 rows of groups of 32)
+  constexpr bool WORDS = GPB > 1;
+  constexpr int SPL = 4 / GPB;  // stages per load of zero points
+  uint64_t zc = 0, zn = 0;      // a byte per group: from this stage on, and the next load's
 #pragma unroll
   for (int i = 0; i < GPB; ++i) nz[i] = 0xE408E408u, nz16[i] = 0xD480D480u;  // zero point 8
   Work w(g);
   while (w.next(g)) {
     const uint8_t *zp = nullptr;
     if (g.zeros) zp = g.zeros + (int64_t)min(w.tile / g.nchunks * BM + row, g.V - 1) * g.ngroups;
+    auto load = [&](int k) {  // of stages [k, k + SPL) (clamped: groups past the end are never used)
+      uint64_t z = 0;
+      if (g.wide_zeros) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(zp + min(k * 2 * GPB, g.ngroups - 8)));
+        z = (uint64_t)x.y << 32 | x.x;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (R::LANES == 1 || ((i / GPB) & 1) == mine)
+            z |= (uint64_t)__ldg(zp + min(k * 2 * GPB + i, g.ngroups - 1)) << (8 * i);
+      }
+      return z;
+    };
+    if (WORDS && zp) {
+      const int k = w.k0 & ~(SPL - 1);
+      zc = load(k), zn = load(k + SPL);
+      zc >>= 16 * GPB * (w.k0 - k);
+    }
     for (int k = w.k0; k < w.k1; ++k) {
       const bool two = 2 * k + 1 < g.nblk;  // (d's last stage may hold one block)
       const uint32_t stage = st.i * (uint32_t)W_BYTES;
-      uint32_t z[GPB];
-      auto fetch = [&](int j) {  // (clamped: groups past the end are never used)
-#pragma unroll
-        for (int i = 0; i < GPB; ++i) z[i] = __ldg(zp + min((2 * k + j) * GPB + i, g.ngroups - 1));
-      };
-      if (zp) fetch(R::LANES == 2 ? mine : 0);
+      uint32_t z = 0;
+      auto fetch = [&](int j) { z = __ldg(zp + min(2 * k + j, g.ngroups - 1)); };  // (with groups of 128)
+      if (!WORDS && zp) fetch(R::LANES == 2 ? mine : 0);
       await(wfull + 8u * st.i, st.parity, late);
 #pragma unroll
       for (int pass = 0; pass < 3 - R::LANES; ++pass) {
@@ -535,7 +556,7 @@ __device__ void expand_rows(const Gemm &g, Sh &sh, const uint8_t *sW, uint32_t t
         if (zp) {
 #pragma unroll
           for (int i = 0; i < GPB; ++i) {
-            const uint32_t zz = (z[i] & 15u) * 0x10001u;
+            const uint32_t zz = ((WORDS ? (uint32_t)(zc >> (8 * (j * GPB + i))) : z) & 15u) * 0x10001u;
             nz[i] = 0xE400E400u | zz, nz16[i] = 0xD400D400u | zz << 4;
           }
         }
@@ -553,13 +574,19 @@ __device__ void expand_rows(const Gemm &g, Sh &sh, const uint8_t *sW, uint32_t t
           tmem_st16(at0 + (uint32_t)j * 128u + (uint32_t)i * 16u, r);
         }
         if (R::LANES == 2 || j == 1 || !two) arrive(wempty + 8u * st.i, lane0);  // (the codes are in registers)
-        if (R::LANES == 1 && j == 0 && two && zp) fetch(1);
+        if (!WORDS && R::LANES == 1 && j == 0 && two && zp) fetch(1);
         tmem_wait_st();
         tc_fence_before();
         arrive(ready + 8u * j, lane0);
       }
       if (late) return raise(g, sh);
       st.next(stages);
+      if (WORDS && zp) {
+        if (SPL == 1 || ((k + 1) & (SPL - 1)) == 0)
+          zc = zn, zn = load(k + 1 + SPL);
+        else
+          zc >>= (16 * GPB) & 63;
+      }
     }
   }
 }
@@ -592,7 +619,7 @@ __device__ __forceinline__ void fma2(float &a0, float &a1, uint32_t x0, uint32_t
 }
 
 // Group sums times scales.
-template <int N, int GPB>
+template <int N, int GPB, bool F32>
 __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
   using R = Roles<N>;
   constexpr int RING = R::RING;
@@ -602,7 +629,14 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
   const int warp = (int)(threadIdx.x >> 5) - R::EXPAND, lane = threadIdx.x & 31;
   const int t = (warp >> 2) & 1, quad = warp & 3, row = t * 128 + quad * 32 + lane, from = (warp >> 3) * NC;
   const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + R::D_COL + (uint32_t)(t * N + from);
-  const bool f32 = g.scale_dtype == MSTAR_DTYPE_F32;
+  // A row's scales lie far from the next row's, so a warp's load touches 32
+  // sectors whatever it takes of each: groups below 128 take SW words of bf16
+  // (two groups each, SPL stages' worth) or a block's groups of f32 at a time
+  // where the rows allow it (64 rows, V=151936, d=2048, groups of 32: 215 us with
+  // single loads, 144 so; with groups of 128 the shifting costs more than the
+  // two loads per stage, 46.1 against 44.4 us for one row).
+  constexpr int SW = N > 64 && GPB < 4 ? 2 : 4, SPL = SW / GPB;
+  constexpr bool WORDS = !F32 && GPB > 1;
   const bool lane0 = lane == 0;
   const uint32_t full = smem_u32(MERGED ? sh.done[t] : sh.dfull[t]);
   const uint32_t ready = smem_u32(sh.ready[t]), dempty = smem_u32(sh.dempty[t]);
@@ -614,19 +648,64 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
   while (w.next(g)) {
     const int v = w.tile / g.nchunks * BM + row, chunk = w.tile % g.nchunks;
     const int64_t s0 = (int64_t)min(v, g.V - 1) * g.ngroups;
-    float acc[NC], s[2][GPB];
+    float acc[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[c] = 0.f;
+    float s[2][WORDS ? 1 : GPB];
+    uint32_t cur[WORDS ? SW : 1], nxt[WORDS ? SW : 1];  // from this stage on, and the next load's
     auto fetch = [&](int j, int b) {  // (clamped: groups past the end are never used)
+      const float *p = static_cast<const float *>(g.scales) + s0;
+      if constexpr (!F32) {
+        s[j][0] = __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(g.scales) + s0 + min(b, g.ngroups - 1)));
+      } else if (GPB > 1 && g.wide_scales) {
+        p += min(b * GPB, g.ngroups - GPB);
+        if constexpr (GPB == 4) {
+          const float4 x = __ldg(reinterpret_cast<const float4 *>(p));
+          s[j][0] = x.x, s[j][1] = x.y, s[j][2] = x.z, s[j][3] = x.w;
+        } else if constexpr (GPB == 2) {
+          const float2 x = __ldg(reinterpret_cast<const float2 *>(p));
+          s[j][0] = x.x, s[j][1] = x.y;
+        }
+      } else {
 #pragma unroll
-      for (int i = 0; i < GPB; ++i) {
-        const int64_t at = s0 + min(b * GPB + i, g.ngroups - 1);
-        s[j][i] = f32 ? __ldg(static_cast<const float *>(g.scales) + at)
-                      : __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(g.scales) + at));
+        for (int i = 0; i < GPB; ++i) s[j][i] = __ldg(p + min(b * GPB + i, g.ngroups - 1));
       }
     };
-    fetch(0, w.b0());
-    fetch(1, w.b0() + 1);
+    auto load = [&](int k, uint32_t (&x)[WORDS ? SW : 1]) {  // of stages [k, k + SPL)
+      if constexpr (WORDS) {
+      const uint16_t *p = static_cast<const uint16_t *>(g.scales) + s0;
+      if (g.wide_scales) {
+        p += min(k * 2 * GPB, g.ngroups - 2 * SW);
+        if constexpr (SW == 4) {
+          const uint4 y = __ldg(reinterpret_cast<const uint4 *>(p));
+          x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+        } else {
+          const uint2 y = __ldg(reinterpret_cast<const uint2 *>(p));
+          x[0] = y.x, x[1] = y.y;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < SW; ++i)
+          x[i] = (uint32_t)__ldg(p + min(k * 2 * GPB + 2 * i, g.ngroups - 1)) |
+                 (uint32_t)__ldg(p + min(k * 2 * GPB + 2 * i + 1, g.ngroups - 1)) << 16;
+      }
+      }
+    };
+    auto step = [&]() {  // to the next stage of a load
+      if constexpr (WORDS) {
+#pragma unroll
+        for (int i = 0; i + GPB < SW; ++i) cur[i] = cur[i + GPB];
+      }
+    };
+    if constexpr (!WORDS) {
+      fetch(0, w.b0());
+      fetch(1, w.b0() + 1);
+    } else {
+      const int k = w.k0 & ~(SPL - 1);
+      load(k, cur);
+      load(k + SPL, nxt);
+      for (int i = k; i < w.k0; ++i) step();
+    }
     for (int k = w.k0; k < w.k1 && !late; ++k) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -655,12 +734,28 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
                              : ready + 8u * (R::LANES == 2 ? j : j == 0 && b + 1 < g.nblk ? 1 : 0),
                      lane0);
             }
+            float scale;
+            if constexpr (!WORDS) {
+              scale = s[j][gi];
+            } else {
+              const int i = j * GPB + gi;
+              scale = __uint_as_float(i & 1 ? cur[i / 2] & 0xFFFF0000u : cur[i / 2] << 16);
+            }
 #pragma unroll
             for (int c = 0; c < LC; c += 2)
-              fma2(acc[c0 + c], acc[c0 + c + 1], r[c / 16][c % 16], r[c / 16][c % 16 + 1], s[j][gi]);
+              fma2(acc[c0 + c], acc[c0 + c + 1], r[c / 16][c % 16], r[c / 16][c % 16 + 1], scale);
           }
         }
-        fetch(j, b + 2);
+        if constexpr (!WORDS) fetch(j, b + 2);
+      }
+      if constexpr (WORDS) {
+        if (((k + 1) & (SPL - 1)) == 0) {
+#pragma unroll
+          for (int i = 0; i < SW; ++i) cur[i] = nxt[i];
+          load(k + 1 + SPL, nxt);
+        } else {
+          step();
+        }
       }
     }
     if (late) raise(g, sh);
@@ -779,7 +874,10 @@ __global__ void __launch_bounds__(Roles<N>::THREADS, 1)
   } else if (warp < FIRST) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R::REGS_SUM));
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    sum_rows<N, GPB>(g, sh, tbase);
+    if (g.scale_dtype == MSTAR_DTYPE_F32)
+      sum_rows<N, GPB, true>(g, sh, tbase);
+    else
+      sum_rows<N, GPB, false>(g, sh, tbase);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::REGS_REST));
     if (warp == FIRST) {
@@ -909,6 +1007,9 @@ static int logits(const void *hidden, int64_t ldh, int B, const mstar_w4_t *w, v
   g.scales = w->scales;
   g.scale_dtype = w->scale_dtype;
   g.zeros = static_cast<const uint8_t *>(w->zeros);
+  // rows of eight groups each way: 16 bytes of scales, 8 of zero points
+  g.wide_scales = g.ngroups % 8 == 0 && reinterpret_cast<uintptr_t>(w->scales) % 16 == 0;
+  g.wide_zeros = g.ngroups % 8 == 0 && reinterpret_cast<uintptr_t>(w->zeros) % 8 == 0;
   g.out = out;
   g.ld = ld;
   g.out_dtype = dtype;

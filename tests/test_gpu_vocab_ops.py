@@ -707,3 +707,30 @@ def test_gradient_of_rows_far_from_zero(dtype):
     x[:, :1000] = -math.inf
     got = k.token_logprobs_grad(x[:, :1000], ids, lse, one)
     assert got[0, 3] == 1 and not bool(got[0, :3].any()) and not bool(got[0, 4:].any())
+
+
+@pytest.mark.parametrize("g", [32, 64, 128])
+@pytest.mark.parametrize("B", [3, 20, 50, 100])
+def test_w4_scales_and_zero_points_at_any_address(B, g):
+    """Rows of scales and zero points that allow wide loads and the same
+    values at odd addresses: equal bits, and the definition's."""
+    from mstar_rs_b200 import kernel as k
+
+    V = 700
+    for d in (1024, 2048, 1024 + 128):
+        hidden = torch.randn(B, d, device="cuda", generator=gen(d)).to(BF16)
+        for stype in (BF16, F32):
+            codes, scales, zeros = w4_inputs(V, d, g, stype, True, B + d)
+
+            def moved(t, by):
+                flat = torch.empty(t.numel() + by, device="cuda", dtype=t.dtype)
+                flat[by:] = t.flatten()
+                return flat[by:].view(t.shape)
+
+            for z in (zeros, None):
+                out = k.lmhead_logits_w4(hidden, codes, scales, zeros=z)
+                ref, tol = R.head(hidden, codes, scales, z, F32, parts=16)
+                near(out, ref, tol)
+                for by in (1, 2):
+                    other = k.lmhead_logits_w4(hidden, codes, moved(scales, by), zeros=None if z is None else moved(z, by))
+                    assert torch.equal(out, other)
