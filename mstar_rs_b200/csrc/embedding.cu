@@ -250,7 +250,7 @@ constexpr int MAX_BINS = SORT_NT;  // ids per CTA of the sort
 constexpr int SUM_NT = 128;
 constexpr int JOIN_G = 8;
 constexpr int MAX_CHUNK = 128;
-constexpr int STAGE_BYTES = 32 * 1024;
+constexpr int STAGE_BYTES = 28 * 1024;  // (seven CTAs of the sums per SM: 1036, one wave of the usual thousand)
 constexpr int LONG_RUN = 32;  // a run of at most this many tokens belongs to the chunk in which it starts
 
 struct Grad {
@@ -440,28 +440,36 @@ __global__ void __launch_bounds__(SUM_NT) sum_tokens_kernel(const Grad a) {
     if (stop - a.start[r] <= LONG_RUN) end = stop - s0;
   }
   if (col >= a.d) return;
-  // A batch of rows is in flight at once: with 16-byte accesses through
-  // asynchronous copies into shared memory (each thread reads back only what
-  // it copied itself), otherwise through registers.
-  constexpr int BATCH = W == 8 ? STAGE_BYTES / (SUM_NT * W * (int)sizeof(TI)) : 8;
+  // A batch of rows is in flight at once, through registers; with 16-byte
+  // accesses through asynchronous copies into shared memory, the next batch
+  // while one is added (each thread reads back only what it copied itself).  30011
+  // tokens of 1024 bf16 over 4099 ids: 59.3 us with one batch of 32 KB, 57.1 so.
+  constexpr int BATCH = W == 8 ? STAGE_BYTES / 2 / (SUM_NT * W * (int)sizeof(TI)) : 8;
   constexpr int PARTS = W * (int)sizeof(TI) / 16;  // 16-byte copies per thread and row
   __shared__ __align__(16) uint8_t stage[W == 8 ? STAGE_BYTES : 16];
   float acc[W] = {}, b[W];
   load_base<TO, W>(a, skey[begin + 1], col, b);  // (read as a run begins: it is there when the run ends)
+  uint8_t *half = stage;  // the batch at hand; the next one lands in the other half
+  auto copy = [&](int s, uint8_t *to) {
+    const int n = min(BATCH, end - s);
+    for (int u = 0; u < n; ++u) {
+      const TI *from = static_cast<const TI *>(a.dout) + (int64_t)spos[s + u] * a.ldo + col;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         smem_u32(to + ((u * PARTS + i) * SUM_NT + (int)threadIdx.x) * 16)),
+                     "l"(reinterpret_cast<const uint4 *>(from) + i)
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (W == 8) copy(begin, half);
   for (int s = begin; s < end; s += BATCH) {
     const int n = min(BATCH, end - s);
     float x[W == 8 ? 1 : BATCH][W];
     if constexpr (W == 8) {
-      for (int u = 0; u < n; ++u) {
-        const TI *from = static_cast<const TI *>(a.dout) + (int64_t)spos[s + u] * a.ldo + col;
-#pragma unroll
-        for (int i = 0; i < PARTS; ++i)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                           smem_u32(stage + ((u * PARTS + i) * SUM_NT + (int)threadIdx.x) * 16)),
-                       "l"(reinterpret_cast<const uint4 *>(from) + i)
-                       : "memory");
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
+      copy(s + BATCH, half == stage ? stage + STAGE_BYTES / 2 : stage);  // (past the end: an empty group)
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
     } else {
 #pragma unroll
       for (int u = 0; u < BATCH; ++u)
@@ -488,11 +496,12 @@ __global__ void __launch_bounds__(SUM_NT) sum_tokens_kernel(const Grad a) {
         float y[8];
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4 *>(stage + ((u * PARTS + i) * SUM_NT + (int)threadIdx.x) * 16);
+          const uint4 w = *reinterpret_cast<const uint4 *>(half + ((u * PARTS + i) * SUM_NT + (int)threadIdx.x) * 16);
           unpack16<TI>(w, y + i * (8 / PARTS));
         }
         take(u, y);
       }
+      half = half == stage ? stage + STAGE_BYTES / 2 : stage;
     } else {
 #pragma unroll
       for (int u = 0; u < BATCH; ++u)
@@ -521,7 +530,8 @@ __global__ void __launch_bounds__(SUM_NT *JOIN_G) join_tokens_kernel(const Grad 
     const int mine = c0 + (int)threadIdx.x * (int)gridDim.x;
     if (mine < full) {
       const int s1 = (mine + 1) * a.chunk, id = a.key[s1 - 1], r = rank_of(a, id), first = a.start[r];
-      if (a.key[s1] == id && first >= mine * a.chunk && a.start[r + 1] - first > LONG_RUN) found[atomicAdd(&nfound, 1)] = mine;
+      if (a.key[s1] == id && first >= mine * a.chunk && a.start[r + 1] - first > LONG_RUN)
+        found[atomicAdd(&nfound, 1)] = mine;
     }
     __syncthreads();
     for (int f = 0; f < nfound; ++f) {  // (their order does not matter: each is an id of its own)
@@ -673,7 +683,9 @@ static int launch_grad(Grad &a, cudaStream_t st) {
 
 template <typename TI, typename TO>
 static int launch_grad_w(Grad &a, int w, cudaStream_t st) {
-  return w == 8 ? launch_grad<TI, TO, 8>(a, st) : w == 2 ? launch_grad<TI, TO, 2>(a, st) : launch_grad<TI, TO, 1>(a, st);
+  return w == 8   ? launch_grad<TI, TO, 8>(a, st)
+         : w == 2 ? launch_grad<TI, TO, 2>(a, st)
+                  : launch_grad<TI, TO, 1>(a, st);
 }
 
 }  // namespace emb
