@@ -309,7 +309,10 @@ __device__ __forceinline__ Scalars scalars(const Args &a, int row, int64_t id, b
   }
   if (MODE == LOGPROBS) return r;
   // lane 0: exp(logp - old) - 1, lane 1: exp(ref - logp) - 1
-  const double q = lane == 1 ? (double)tok.ref_logp - lp : a.old_logp ? lp - (double)tok.old_logp : isnan(lp) ? lp : 0.0;
+  const double q = lane == 1       ? (double)tok.ref_logp - lp
+                   : a.old_logp ? lp - (double)tok.old_logp
+                   : isnan(lp)  ? lp
+                                : 0.0;
   const double e = expm1(q);
   const double ratio = 1.0 + __shfl_sync(~0u, e, 0), eq = __shfl_sync(~0u, e, 1), qq = __shfl_sync(~0u, q, 1);
   double loss = 0.0, d = 0.0;
