@@ -784,10 +784,14 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
     int c_lo, c_hi;
     sharers(g, again.tile, c_lo, c_hi);
     const int chunk = again.tile % g.nchunks, cols = min(g.rows, g.B - chunk * g.rows);
-    constexpr int JC = NC < 128 ? 16 : 32;  // columns at a time
+    // columns at a time, and parts: with more of either the wide sizes spill and
+    // the narrow ones lose registers elsewhere (128 rows, V=4099, d=1024: 30.7 us
+    // with one part at a time, 29.4 with two, 34.0 with four)
+    constexpr int JC = NC < 128 ? 16 : 32, JP = NC < 128 ? 1 : 2;
 #pragma unroll 1
     for (int c0 = from; c0 < min(cols, from + NC); c0 += JC) {
       float sum[JC] = {};
+#pragma unroll JP
       for (int q = c_lo; q < c_hi; ++q) {
         const float *p = g.parts + ((size_t)q * 2 + (unit_start(g, q) <= first ? 1 : 0)) * (size_t)g.n * BM + row;
         float x[JC];  // (columns past the last read it again: no load waits for another)
