@@ -915,12 +915,24 @@ static Gemm plan(int B, int V, int d) {
   g.B = B;
   g.V = V;
   g.d = d;
-  g.nchunks = (B + MAX_N - 1) / MAX_N;
-  g.rows = (B + g.nchunks - 1) / g.nchunks;
-  g.n = (g.rows + 15) & ~15;
   g.nks = (d + KS - 1) / KS;
   g.nblk = (d + KB - 1) / KB;
-  g.ntt = (V + BM - 1) / BM * g.nchunks;
+  const int tiles = (V + BM - 1) / BM;
+  g.nchunks = (B + MAX_N - 1) / MAX_N;
+  // Chunks of up to 128 rows read and expand each code least often, but their
+  // blocks take turns in one accumulator and their shared tiles are long to add.
+  // With few units per SM narrower chunks win: 64 rows while that makes at most
+  // 16 units per SM (128 rows, groups of 128, d=2048: V=16384 41 -> 27 us, V=32000
+  // 54 -> 42; at V=50000 they would gain too, 69 -> 57, but with groups of 32 and
+  // d=4096 lose, 112 -> 123), down to 16 rows while at most 4 (128 rows, d=1024,
+  // V=4099: 29 -> 16 us; at 6, V=8192, d=2048, groups of 64: 25 -> 28).
+  const int64_t units = (int64_t)tiles * g.nks, sms = sm_count();
+  if (units * ((B + 63) / 64) <= 16 * sms) g.nchunks = (B + 63) / 64;
+  g.nchunks = (int)std::max<int64_t>(g.nchunks, std::min<int64_t>(4 * sms / units, (B + 15) / 16));
+  g.rows = (B + g.nchunks - 1) / g.nchunks;
+  g.nchunks = (B + g.rows - 1) / g.rows;
+  g.n = (g.rows + 15) & ~15;
+  g.ntt = tiles * g.nchunks;
   // (64 rows, V=151936, d=2048: 83 us with three hidden stages, 77 with four)
   g.hstages = g.n <= 16 ? 8 : g.n <= 32 ? 6 : g.n <= 64 ? 4 : 3;
   g.wstages = std::min(MAX_WS, (SMEM_BUDGET - g.hstages * g.n * KB * 2) / W_BYTES);

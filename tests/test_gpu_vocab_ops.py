@@ -734,3 +734,21 @@ def test_w4_scales_and_zero_points_at_any_address(B, g):
                 for by in (1, 2):
                     other = k.lmhead_logits_w4(hidden, codes, moved(scales, by), zeros=None if z is None else moved(z, by))
                     assert torch.equal(out, other)
+
+
+@pytest.mark.parametrize("V,d", [(300, 256), (1302, 1280), (4099, 1024), (12000, 1024), (33000, 512)])
+def test_w4_chunks_of_rows(V, d):
+    """Batches around every chunk's width, over matrices of few and many
+    units, against the definition; nothing beyond their rows and columns is
+    written."""
+    from mstar_rs_b200 import kernel as k
+
+    codes, scales, zeros = w4_inputs(V, d, 64, BF16, True, V)
+    hidden = torch.randn(256, d, device="cuda", generator=gen(d)).to(BF16)
+    ref, tol = R.head(hidden, codes, scales, zeros, F32, parts=16)
+    for B in (15, 16, 17, 31, 33, 48, 63, 65, 127, 129, 191, 193, 255, 256):
+        rows = torch.arange(256, device="cuda")[-B:]
+        out = torch.full((B + 1, V + 3), 7.0, device="cuda")
+        got = k.lmhead_logits_w4(hidden[rows], codes, scales, zeros=zeros, out=out[:B, :V])
+        near(got, ref[rows], tol[rows])
+        assert bool((out[B] == 7).all()) and bool((out[:, V:] == 7).all())
