@@ -33,7 +33,7 @@
 // instructions and an arrival cost each role some hundred cycles, next to the
 // 735 in which memory delivers a block of 256 x 128 codes.  So the two blocks
 // of a stage have an A buffer, accumulators, expander warps and issuers of
-// their own (up to 64 batch rows), each of which has twice the time; with
+// their own (up to 32 batch rows), each of which has twice the time; with
 // groups of 128 one barrier says that A is written and the accumulator free,
 // and one that both are done with.
 //

@@ -752,3 +752,25 @@ def test_w4_chunks_of_rows(V, d):
         got = k.lmhead_logits_w4(hidden[rows], codes, scales, zeros=zeros, out=out[:B, :V])
         near(got, ref[rows], tol[rows])
         assert bool((out[B] == 7).all()) and bool((out[:, V:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_policy_loss_leaves_lse(dtype):
+    """The C entry's lse is token_logprobs' (0 for padding rows)."""
+    import ctypes
+
+    from mstar_rs_b200 import _native as N
+    from mstar_rs_b200 import kernel as k
+
+    n, V = 5, 777
+    x = torch.randn(n, V, device="cuda", generator=gen(1)).to(dtype)
+    x[2] = -math.inf
+    ids = torch.tensor([3, -1, 4, V, 5], device="cuda")
+    adv = torch.ones(n, device="cuda")
+    loss, logp, lse = (torch.full((n,), 9.0, device="cuda") for _ in range(3))
+    p = N.PolicyParams(x.data_ptr(), N.DTYPE_F32 if dtype == F32 else N.DTYPE_BF16, n, V, 0, V, ids.data_ptr(), None, None,
+                       adv.data_ptr(), None, 1.0, 0.2, 0.2, 0.0, loss.data_ptr(), logp.data_ptr(), lse.data_ptr(), None,
+                       0, None)
+    k._call(x.device, "mstar_policy_loss", ctypes.byref(p))
+    want_logp, want = k.token_logprobs(x, ids)
+    assert torch.equal(lse, torch.where((ids >= 0) & (ids < V), want, 0.0)) and torch.equal(logp, want_logp)
