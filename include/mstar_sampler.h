@@ -271,7 +271,8 @@ typedef struct mstar_w4 {
  * fp32), stored as dtype.  Each hidden row enters as fp16 times a power of two:
  * exact for values down to 2^-32 of its largest, below that off by at most
  * 2^-40 of it.  NaN and infinities go where the products take them.  B <= 256.  workspace: device scratch of at least
- * mstar_lmhead_w4_workspace_bytes(B, V, d) bytes, 256-byte aligned; its
+ * mstar_lmhead_w4_workspace_bytes(B, V, d) bytes (which grow with B: the largest
+ * batch's serves the smaller ones), 256-byte aligned; its
  * contents need not be preserved or initialised, and calls that overlap on
  * the GPU need their own.  status: NULL or a device word that gets bit 1 if
  * a bounded in-kernel wait ran out. */

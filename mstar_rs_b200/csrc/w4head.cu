@@ -953,12 +953,16 @@ static int grid_of(const Gemm &g) {
 }
 
 // Workspace: arrival counters, the hidden rows as operands, their scales, the
-// parts of shared tiles; each rounded to 256 bytes.
+// parts of shared tiles; each rounded to 256 bytes.  Sized by what any batch of
+// up to B rows may take (the chunks' width goes up and down with B), so that a
+// workspace for the largest batch serves the smaller ones.
 static int64_t up(int64_t b) { return (b + 255) / 256 * 256; }
-static int64_t hidden_at(const Gemm &g) { return up((int64_t)g.ntt * 4); }
+static int64_t hidden_at(const Gemm &g) { return up((int64_t)((g.V + BM - 1) / BM) * ((g.B + 15) / 16) * 4); }
 static int64_t scale_at(const Gemm &g) { return hidden_at(g) + up((int64_t)g.B * g.d * 2); }
 static int64_t parts_at(const Gemm &g) { return scale_at(g) + up((int64_t)g.B * 4); }
-static int64_t workspace_bytes(const Gemm &g) { return parts_at(g) + (int64_t)grid_of(g) * 2 * g.n * BM * 4; }
+static int64_t workspace_bytes(const Gemm &g) {
+  return parts_at(g) + (int64_t)sm_count() * 2 * std::min(MAX_N, (g.B + 15) / 16 * 16) * BM * 4;
+}
 
 static int check_sizes(int B, int V, int d) {
   if (B < 1 || B > MAX_B) return fail(MSTAR_ERR_INVALID, "B must be in [1, 256]");

@@ -774,3 +774,18 @@ def test_policy_loss_leaves_lse(dtype):
     k._call(x.device, "mstar_policy_loss", ctypes.byref(p))
     want_logp, want = k.token_logprobs(x, ids)
     assert torch.equal(lse, torch.where((ids >= 0) & (ids < V), want, 0.0)) and torch.equal(logp, want_logp)
+
+
+@pytest.mark.parametrize("V,d", [(1302, 1280), (4099, 1024), (33000, 512)])
+def test_w4_one_workspace_for_all_batches(V, d):
+    """The largest batch's scratch, full of ones before each call, serves the
+    smaller batches: the same bits as with fresh scratch."""
+    from mstar_rs_b200 import kernel as k
+
+    codes, scales, _ = w4_inputs(V, d, 64, BF16, False, V)
+    hidden = torch.randn(200, d, device="cuda", generator=gen(d)).to(BF16)
+    ws = k.lmhead_w4_workspace(200, V, d, "cuda")
+    for B in (200, 129, 128, 65, 64, 33, 16, 1):
+        ws.fill_(255)
+        got = k.lmhead_logits_w4(hidden[:B], codes, scales, workspace=ws)
+        assert torch.equal(got, k.lmhead_logits_w4(hidden[:B], codes, scales))

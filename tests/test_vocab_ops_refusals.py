@@ -211,3 +211,10 @@ def test_quantize_w4(group, zero_points, sdt):
         kernel.quantize_w4(w[0])
     with pytest.raises(TypeError):
         kernel.quantize_w4(w, scale_dtype=torch.float16)
+
+
+@pytest.mark.parametrize("V,d", [(300, 256), (4099, 1024), (2048, 4096), (32000, 2048), (151936, 2048)])
+def test_w4_workspace_of_a_larger_batch_serves_smaller_ones(V, d):
+    lib = N.lib()
+    sizes = [lib.mstar_lmhead_w4_workspace_bytes(B, V, d) for B in range(1, 257)]
+    assert sizes[0] > 0 and all(a <= b for a, b in zip(sizes, sizes[1:]))
