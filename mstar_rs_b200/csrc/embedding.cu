@@ -635,7 +635,11 @@ static Layout layout(int N, int V, int d) {
   l.pos = up((((int64_t)sort_bins(V) << sort_log2(V)) + 1) * 4);
   l.key = l.pos + up((int64_t)N * 4);
   l.part = l.key + up((int64_t)N * 4);
-  l.bytes = l.part + up((int64_t)l.nchunks * 2 * d * 4);
+  // parts: as many as any batch of up to N tokens has (the chunks' length grows
+  // with N between 32 and 128, where their number stays near 2368 / tiles), so
+  // that a workspace for the largest batch serves the smaller ones
+  const int64_t most = std::min<int64_t>((N + 31) / 32, std::max<int64_t>(2442 / tiles + 3, (N + 127) / 128));
+  l.bytes = l.part + up(std::max<int64_t>(most, l.nchunks) * 2 * d * 4);
   return l;
 }
 

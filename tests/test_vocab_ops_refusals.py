@@ -218,3 +218,11 @@ def test_w4_workspace_of_a_larger_batch_serves_smaller_ones(V, d):
     lib = N.lib()
     sizes = [lib.mstar_lmhead_w4_workspace_bytes(B, V, d) for B in range(1, 257)]
     assert sizes[0] > 0 and all(a <= b for a, b in zip(sizes, sizes[1:]))
+
+
+@pytest.mark.parametrize("d", [1, 513, 1024, 2048, 5000, 65536])
+def test_embed_grad_workspace_of_more_tokens_serves_fewer(d):
+    lib = N.lib()
+    counts = list(range(1, 4000)) + list(range(4000, 400000, 37))
+    sizes = [lib.mstar_embed_grad_workspace_bytes(n, 4099, d) for n in counts]
+    assert sizes[0] > 0 and all(a <= b for a, b in zip(sizes, sizes[1:]))
