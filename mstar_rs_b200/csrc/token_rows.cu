@@ -445,6 +445,9 @@ __global__ void __launch_bounds__(NT, 6) token_rows_kernel(const Args a) {
   __syncthreads();
   auto load = [&](int v) { return __ldcs(in.vecs() + v); };
   if (sh.row.exact) {  // the row's largest value is at the edge of the type (or nothing is left of it)
+    // A maximum passes over NaN: a row of -inf alone and one of NaN and -inf both
+    // have -inf.  The sum tells them apart (0 and NaN; warp 0 holds it).
+    const bool nan = isnan(t.y);
     float m = fringe >= 0 ? x_fringe : -INFINITY;
     for (int v = v0 + tid; v < v1; v += NT) m = fmaxf(m, Vec<T>::largest(load(v)));
     m = cluster_join<1>(sh, S, rank, m, 0.f, false).x;
@@ -460,7 +463,7 @@ __global__ void __launch_bounds__(NT, 6) token_rows_kernel(const Args a) {
     }
     t = cluster_join<2>(sh, S, rank, 0.f, s, false);
     if (tid < 32) {
-      Scalars r = scalars<MODE>(a, row, id, ok, (double)m, t.y, m == -INFINITY, tok, rank == 0);
+      Scalars r = scalars<MODE>(a, row, id, ok, (double)m, t.y, m == -INFINITY && !nan, tok, rank == 0);
       r.M = m;
       r.exact = 1;
       if (tid == 0) sh.row = r;

@@ -789,3 +789,42 @@ def test_w4_one_workspace_for_all_batches(V, d):
         ws.fill_(255)
         got = k.lmhead_logits_w4(hidden[:B], codes, scales, workspace=ws)
         assert torch.equal(got, k.lmhead_logits_w4(hidden[:B], codes, scales))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [5, 1000, 40000])
+def test_rows_without_a_number(V, dtype):
+    """Rows of NaN alone, and of NaN among masked ids, are NaN and not empty:
+    their log-probabilities, losses and gradients say so.  Padding rows among
+    them stay zero and empty rows empty."""
+    from mstar_rs_b200 import _native as N
+    from mstar_rs_b200 import kernel
+
+    x = torch.full((7, V), -math.inf, device="cuda").to(dtype)
+    x[0] = math.nan
+    x[1, V - 1] = math.nan             # behind the aligned vectors, or in the last of them
+    x[2, 0] = math.nan
+    x[3] = torch.finfo(dtype).min
+    x[3, 1] = math.nan                 # beside the type's lowest value
+    x[4] = math.nan                    # padding
+    x[6, V // 2] = math.nan            # (row 5 is empty)
+    ids = torch.tensor([2, 2, 0, 2, -1, 2, V // 2], device="cuda")
+    nan = torch.tensor([True, True, True, True, False, False, True], device="cuda")
+    for T in (1.0, 1e-5, 1e5):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        logp, lse = kernel.token_logprobs(x[nan], ids[nan], temperature=T, status=status)
+        assert status.item() == 0 and bool(logp.isnan().all()) and bool(lse.isnan().all())
+        logp, lse = kernel.token_logprobs(x, ids, temperature=T)
+        assert torch.equal(logp.isnan(), nan) and logp[4] == 0 and logp[5] == -math.inf and lse[5] == -math.inf
+        one = torch.ones(7, device="cuda")
+        g = kernel.token_logprobs_grad(x, ids, lse, one, temperature=T)
+        assert bool(g[nan].isnan().all()) and not bool(g[4:6].any())
+        for old in (None, one):
+            for adv in (one, -one, 0 * one):
+                status.zero_()
+                loss, lp, dx = kernel.policy_loss(x, ids, old, adv, ref_logp=one, kl_coef=0.1, temperature=T, status=status)
+                assert status.item() == N.STATUS_EMPTY
+                assert torch.equal(lp.isnan(), nan) and torch.equal(loss.isnan(), nan) and not bool(loss[4:6].any())
+                assert bool(dx[nan].isnan().all()) and not bool(dx[4:6].any())
+                value = kernel.policy_loss(x, ids, old, adv, ref_logp=one, kl_coef=0.1, temperature=T, grad=False)[0]
+                assert torch.equal(value.isnan(), nan)
