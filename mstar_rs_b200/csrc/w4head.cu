@@ -59,6 +59,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "ring.cuh"
 #include "tcgen05.cuh"
 
 namespace mstar {
@@ -217,14 +218,6 @@ __device__ __forceinline__ void arrive(uint32_t bar, bool lane0) {
   if (lane0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// A place in a ring of `n` stages and the parity of its current use.
-struct Ring {
-  uint32_t i = 0, parity = 0;
-  __device__ __forceinline__ void next(uint32_t n) {
-    if (++i == n) i = 0, parity ^= 1u;
-  }
-};
-
 // Named barriers 1 and 2 tell the counting warp that a part of this CTA's two
 // shared tiles is written (the accumulator warps arrive and go on); barrier 3
 // tells them what it counted.
@@ -357,12 +350,13 @@ __global__ void __launch_bounds__(PREP_NT)
   }
 }
 
-// Waits until each of the ring's last `n` uses (at most its stages) has landed.
-__device__ void drain(const Gemm &g, Sh &sh, uint64_t *full, Ring r, uint32_t n, uint32_t stages) {
+// Waits until each of a ring's last `n` uses (at most its `stages`, which are
+// `step` apart) has landed.
+__device__ void drain(const Gemm &g, Sh &sh, uint64_t *full, Ring r, uint32_t n, uint32_t stages, uint32_t step = 1) {
   for (uint32_t j = 0; j < n; ++j) {
     if (r.i == 0) r.i = stages, r.parity ^= 1u;
     --r.i;
-    if (!mbar_wait(&full[r.i], r.parity)) raise(g, sh);
+    if (!mbar_wait(&full[r.i * step], r.parity)) raise(g, sh);
   }
 }
 
@@ -391,30 +385,42 @@ __device__ void produce_weights(const Gemm &g, Sh &sh, uint8_t *sW, const CUtens
   drain(g, sh, sh.wfull, r, used, stages);
 }
 
+template <int N>
 __device__ void produce_hidden(const Gemm &g, Sh &sh, uint8_t *sH, const CUtensorMap *map) {
+  constexpr int LANES = Roles<N>::LANES;
   const uint64_t pol = policy_evict_last();
-  const uint32_t stages = (uint32_t)g.hstages, box = (uint32_t)g.n * 128u;
-  Ring r;
-  uint32_t used = 0;
+  const uint32_t stages = (uint32_t)g.hstages, per = stages / LANES, box = (uint32_t)g.n * 128u;
+  LaneRings<LANES> r;
+  uint32_t used[LANES] = {};
   Work w(g);
   bool go = true;
   while (go && w.next(g)) {
     const int y = w.tile % g.nchunks * g.rows, b1 = w.b1(g);
     for (int b = w.b0(); b < b1; ++b) {
-      if (aborted(sh) || (used == stages && !mbar_wait(&sh.hempty[r.i], r.parity ^ 1u))) {
+      const bool second = LANES == 2 && (b & 1);  // (selects: an index would put the rings into local memory)
+      const uint32_t at = second ? r.stage(LANES - 1) : r.stage(0), u = second ? used[LANES - 1] : used[0];
+      const uint32_t parity = second ? r.parity(LANES - 1) : r.parity(0);
+      if (aborted(sh) || (u == per && !mbar_wait(&sh.hempty[at], parity ^ 1u))) {
         go = false;
         break;
       }
-      mbar_expect_tx(&sh.hfull[r.i], 2u * box);
-      uint8_t *to = sH + r.i * 2u * box;
-      tma_load_2d(to, map, b * KB, y, &sh.hfull[r.i], pol);
-      tma_load_2d(to + box, map, b * KB + 64, y, &sh.hfull[r.i], pol);
-      r.next(stages);
-      used = min(used + 1, stages);
+      mbar_expect_tx(&sh.hfull[at], 2u * box);
+      uint8_t *to = sH + at * 2u * box;
+      tma_load_2d(to, map, b * KB, y, &sh.hfull[at], pol);
+      tma_load_2d(to + box, map, b * KB + 64, y, &sh.hfull[at], pol);
+      if (second) {
+        r.next(LANES - 1, stages);
+        used[LANES - 1] = min(u + 1, per);
+      } else {
+        r.next(0, stages);
+        used[0] = min(u + 1, per);
+      }
     }
   }
   if (!go) raise(g, sh);
-  drain(g, sh, sh.hfull, r, used, stages);
+#pragma unroll
+  for (int lane = 0; lane < LANES; ++lane)
+    drain(g, sh, sh.hfull + lane, r.ring[lane], used[lane], per, (uint32_t)LANES);
 }
 
 // MMAs of half t of the tile, of the blocks of `lane` (with one lane: of all).
@@ -432,7 +438,7 @@ __device__ void issue(const Gemm &g, Sh &sh, uint8_t *sH, uint32_t tbase, int wh
   const uint32_t hfull = smem_u32(sh.hfull), hempty = smem_u32(sh.hempty);
   const uint32_t ready = smem_u32(sh.ready[t]), done = smem_u32(sh.done[t]);
   const uint32_t dfull = smem_u32(sh.dfull[t]), dempty = smem_u32(sh.dempty[t]);
-  Ring h;
+  LaneRings<R::LANES> h;
   uint32_t rp = 0, dp = 0, fresh = 0xFu;  // parities of ready[t][j] and dempty[t][slot], a bit each; unused slots
   int slot = 0;                           // within the lane's ring
   uint32_t late = 0;
@@ -442,14 +448,13 @@ __device__ void issue(const Gemm &g, Sh &sh, uint8_t *sH, uint32_t tbase, int wh
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (j == 1 && 2 * k + 1 >= g.nblk) break;
-        if (R::LANES == 2 && j != lane) {
-          h.next(hstages);
-          continue;
-        }
-        await(hfull + 8u * h.i, h.parity, late);
+        if (R::LANES == 2 && j != lane) continue;
+        const int own = R::LANES == 2 ? j : 0;
+        const uint32_t at = h.stage(own);
+        await(hfull + 8u * at, h.parity(own), late);
         await(ready + 8u * j, (rp >> j) & 1u, late);
         rp ^= 1u << j;
-        const uint32_t lo = hlo + h.i * 2u * box16, aj = a0 + (uint32_t)j * 128u;
+        const uint32_t lo = hlo + at * 2u * box16, aj = a0 + (uint32_t)j * 128u;
         if (MERGED) {
           tc_fence_after();
           mma_group<KB>(lead, d0 + (R::LANES == 2 ? j : 0) * 2u * N, aj, lo, hhi, box16, idesc);
@@ -471,8 +476,8 @@ __device__ void issue(const Gemm &g, Sh &sh, uint8_t *sH, uint32_t tbase, int wh
           }
         }
         commit(lead, done + 8u * j);
-        commit(lead, hempty + 8u * h.i);
-        h.next(hstages);
+        commit(lead, hempty + 8u * at);
+        h.next(own, hstages);
       }
     }
   }
@@ -889,7 +894,7 @@ __global__ void __launch_bounds__(Roles<N>::THREADS, 1)
     } else if (warp == FIRST + 1) {
       asm volatile("griddepcontrol.wait;" ::: "memory");
       asm volatile("fence.proxy.async;" ::: "memory");
-      if (lane == 0) produce_hidden(g, sh, sH, &th);
+      if (lane == 0) produce_hidden<N>(g, sh, sH, &th);
     } else if (warp < FIRST + 2 + R::ISSUE) {
       issue<N, GPB>(g, sh, sH, tbase, warp - FIRST - 2);
     }
@@ -933,7 +938,8 @@ static Gemm plan(int B, int V, int d) {
   g.nchunks = (B + g.rows - 1) / g.rows;
   g.n = (g.rows + 15) & ~15;
   g.ntt = tiles * g.nchunks;
-  // (64 rows, V=151936, d=2048: 83 us with three hidden stages, 77 with four)
+  // (64 rows, V=151936, d=2048: 83 us with three hidden stages, 77 with four; a
+  // multiple of the lanes that Roles gives each width)
   g.hstages = g.n <= 16 ? 8 : g.n <= 32 ? 6 : g.n <= 64 ? 4 : 3;
   g.wstages = std::min(MAX_WS, (SMEM_BUDGET - g.hstages * g.n * KB * 2) / W_BYTES);
   return g;

@@ -828,3 +828,22 @@ def test_rows_without_a_number(V, dtype):
                 assert bool(dx[nan].isnan().all()) and not bool(dx[4:6].any())
                 value = kernel.policy_loss(x, ids, old, adv, ref_logp=one, kl_coef=0.1, temperature=T, grad=False)[0]
                 assert torch.equal(value.isnan(), nan)
+
+
+@pytest.mark.parametrize("g", [32, 64, 128])
+@pytest.mark.parametrize("V,d", [(2000, 128), (70000, 384), (9001, 640), (40000, 1152)])
+def test_w4_odd_numbers_of_blocks(V, d, g):
+    """Widths of an odd number of 128-column blocks, where the blocks of one
+    tile end in the middle of a stage, over one and many tiles per CTA."""
+    from mstar_rs_b200 import kernel as k
+
+    codes, scales, zeros = w4_inputs(V, d, g, BF16, True, V)
+    hidden = torch.randn(64, d, device="cuda", generator=gen(d)).to(BF16)
+    ref, tol = R.head(hidden, codes, scales, zeros, F32, parts=16)
+    for B in (1, 16, 17, 32, 64):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        first = k.lmhead_logits_w4(hidden[:B], codes, scales, zeros=zeros, status=status)
+        near(first, ref[:B], tol[:B])
+        for _ in range(3):
+            assert torch.equal(first, k.lmhead_logits_w4(hidden[:B], codes, scales, zeros=zeros, status=status))
+        assert status.item() == 0
