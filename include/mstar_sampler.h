@@ -44,7 +44,8 @@ extern "C" {
 #define MSTAR_FLAG_ADVANCE_OFFSET 0x4u /* offset[slot] += 1 after the draw */
 #define MSTAR_FLAG_FORCE_GENERAL 0x8u  /* testing: take the multi-round selection path */
 #define MSTAR_FLAG_TEST_WITHHOLD 0x10u /* testing: leave each CTA's last bulk copy unissued, so its
-                                          bounded wait (2 ms) runs out: MSTAR_STATUS_TIMEOUT */
+                                          bounded wait (2 ms) runs out: MSTAR_STATUS_TIMEOUT
+                                          (mstar_sampler_lmhead_step_w4: the head's last copy too) */
 
 /* per-row status bits written to out_status */
 #define MSTAR_STATUS_EMPTY 0x1u        /* no token had positive weight; id 0 returned */
@@ -274,8 +275,9 @@ typedef struct mstar_w4 {
  * mstar_lmhead_w4_workspace_bytes(B, V, d) bytes (which grow with B: the largest
  * batch's serves the smaller ones), 256-byte aligned; its
  * contents need not be preserved or initialised, and calls that overlap on
- * the GPU need their own.  status: NULL or a device word that gets bit 1 if
- * a bounded in-kernel wait ran out. */
+ * the GPU need their own.  status: NULL or a device word that gets bit 1 if a
+ * bounded in-kernel wait (0.1 s) ran out: some logits are then wrong or not
+ * written, and nothing else says so. */
 int64_t mstar_lmhead_w4_workspace_bytes(int32_t B, int32_t V, int32_t d);
 int mstar_lmhead_logits_w4(const void *hidden, int64_t ld_hidden, int32_t B, const mstar_w4_t *w, void *logits,
                            int32_t dtype, int64_t ld, void *workspace, int64_t workspace_bytes, uint32_t *status,

@@ -126,6 +126,7 @@ struct Gemm {
   int64_t ld;
   int out_dtype;
   uint32_t *err;
+  int withhold;           // testing: each CTA's last copy of hidden rows is never issued
   const float *row_scale; // [B] what the hidden rows were divided by
   uint32_t *counters;     // [ntt] parts of a shared tile that have arrived
   float *parts;           // [grid][2][n][BM]
@@ -199,9 +200,10 @@ __device__ __forceinline__ void raise(const Gemm &g, Sh &sh) {
 // The hot loops name barriers by their shared-memory address and keep what a
 // hand-over costs to a few instructions: a pipeline of waits is bound by them.
 //
-// Waits for phase `parity`, at most LOOKS looks at the barrier (each of which
-// may sleep until the phase ends; some ten milliseconds in all, and no
-// less than one), and sets `late` if they run out.
+// Waits for phase `parity`, at most LOOKS looks at the barrier, and sets `late` if
+// they run out.  A look sleeps until the phase ends or some 1.5 us have passed
+// (measured): 0.1 s in all, where a stage takes microseconds.  Looks are counted
+// and not time, since a clock runs on while another process has the GPU.
 constexpr uint32_t LOOKS = 1u << 16;
 __device__ __forceinline__ void await(uint32_t bar, uint32_t parity, uint32_t &late) {
   asm volatile(
@@ -352,26 +354,31 @@ __global__ void __launch_bounds__(PREP_NT)
 
 // Waits until each of a ring's last `n` uses (at most its `stages`, which are
 // `step` apart) has landed.
-__device__ void drain(const Gemm &g, Sh &sh, uint64_t *full, Ring r, uint32_t n, uint32_t stages, uint32_t step = 1) {
+__device__ void drain(const Gemm &g, Sh &sh, uint32_t full, Ring r, uint32_t n, uint32_t stages, uint32_t step = 1) {
+  uint32_t late = 0;
   for (uint32_t j = 0; j < n; ++j) {
     if (r.i == 0) r.i = stages, r.parity ^= 1u;
     --r.i;
-    if (!mbar_wait(&full[r.i * step], r.parity)) raise(g, sh);
+    await(full + 8u * r.i * step, r.parity, late);
   }
+  if (late) raise(g, sh);
 }
 
 __device__ void produce_weights(const Gemm &g, Sh &sh, uint8_t *sW, const CUtensorMap *map) {
   // one chunk: every weight is read once; several: their CTAs meet in L2
   const uint64_t pol = g.nchunks == 1 ? policy_evict_first() : policy_evict_last();
-  const uint32_t stages = (uint32_t)g.wstages;
+  const uint32_t stages = (uint32_t)g.wstages, wempty = smem_u32(sh.wempty);
   Ring r;
   uint32_t used = 0;  // stages filled so far, up to the ring's length
+  uint32_t late = 0;
   Work w(g);
   bool go = true;
   while (go && w.next(g)) {
     const int y = w.tile / g.nchunks * BM;
     for (int k = w.k0; k < w.k1; ++k) {
-      if (aborted(sh) || (used == stages && !mbar_wait(&sh.wempty[r.i], r.parity ^ 1u))) {
+      const bool stop = aborted(sh);
+      if (used == stages) await(wempty + 8u * r.i, r.parity ^ 1u, late);
+      if (late || stop) {
         go = false;
         break;
       }
@@ -382,7 +389,7 @@ __device__ void produce_weights(const Gemm &g, Sh &sh, uint8_t *sW, const CUtens
     }
   }
   if (!go) raise(g, sh);
-  drain(g, sh, sh.wfull, r, used, stages);
+  drain(g, sh, smem_u32(sh.wfull), r, used, stages);
 }
 
 template <int N>
@@ -391,16 +398,24 @@ __device__ void produce_hidden(const Gemm &g, Sh &sh, uint8_t *sH, const CUtenso
   const uint64_t pol = policy_evict_last();
   const uint32_t stages = (uint32_t)g.hstages, per = stages / LANES, box = (uint32_t)g.n * 128u;
   LaneRings<LANES> r;
-  uint32_t used[LANES] = {};
+  uint32_t used[LANES] = {}, late = 0;
+  const uint32_t hempty = smem_u32(sh.hempty);
   Work w(g);
   bool go = true;
   while (go && w.next(g)) {
-    const int y = w.tile % g.nchunks * g.rows, b1 = w.b1(g);
+    const int y = w.tile % g.nchunks * g.rows;
+    int b1 = w.b1(g);
+    if (g.withhold) {
+      Work rest = w;
+      b1 -= !rest.next(g);
+    }
     for (int b = w.b0(); b < b1; ++b) {
       const bool second = LANES == 2 && (b & 1);  // (selects: an index would put the rings into local memory)
       const uint32_t at = second ? r.stage(LANES - 1) : r.stage(0), u = second ? used[LANES - 1] : used[0];
       const uint32_t parity = second ? r.parity(LANES - 1) : r.parity(0);
-      if (aborted(sh) || (u == per && !mbar_wait(&sh.hempty[at], parity ^ 1u))) {
+      const bool stop = aborted(sh);
+      if (u == per) await(hempty + 8u * at, parity ^ 1u, late);
+      if (late || stop) {
         go = false;
         break;
       }
@@ -420,7 +435,7 @@ __device__ void produce_hidden(const Gemm &g, Sh &sh, uint8_t *sH, const CUtenso
   if (!go) raise(g, sh);
 #pragma unroll
   for (int lane = 0; lane < LANES; ++lane)
-    drain(g, sh, sh.hfull + lane, r.ring[lane], used[lane], per, (uint32_t)LANES);
+    drain(g, sh, smem_u32(sh.hfull + lane), r.ring[lane], used[lane], per, (uint32_t)LANES);
 }
 
 // MMAs of half t of the tile, of the blocks of `lane` (with one lane: of all).
@@ -1021,7 +1036,7 @@ static int launch_n(const CUtensorMap &tw, const CUtensorMap &th, const Gemm &g,
 }
 
 static int logits(const void *hidden, int64_t ldh, int B, const mstar_w4_t *w, void *out, int dtype, int64_t ld,
-                  void *ws, int64_t ws_bytes, uint32_t *err, cudaStream_t st) {
+                  void *ws, int64_t ws_bytes, uint32_t *err, bool withhold, cudaStream_t st) {
   int rc = check_w4(w);
   if (rc || (rc = check_sizes(B, w->V, w->d))) return rc;
   if (!hidden || !out || !ws) return fail(MSTAR_ERR_INVALID, "hidden, logits and workspace must not be NULL");
@@ -1051,6 +1066,7 @@ static int logits(const void *hidden, int64_t ldh, int B, const mstar_w4_t *w, v
   g.ld = ld;
   g.out_dtype = dtype;
   g.err = err;
+  g.withhold = withhold;
   g.counters = reinterpret_cast<uint32_t *>(p);
   g.parts = reinterpret_cast<float *>(p + parts_at(g));
   void *perm = p + hidden_at(g);
@@ -1101,7 +1117,7 @@ int64_t mstar_lmhead_w4_workspace_bytes(int32_t B, int32_t V, int32_t d) {
 int mstar_lmhead_logits_w4(const void *hidden, int64_t ld_hidden, int32_t B, const mstar_w4_t *w, void *logits,
                            int32_t dtype, int64_t ld, void *workspace, int64_t workspace_bytes, uint32_t *status,
                            void *stream) {
-  return w4::logits(hidden, ld_hidden, B, w, logits, dtype, ld, workspace, workspace_bytes, status,
+  return w4::logits(hidden, ld_hidden, B, w, logits, dtype, ld, workspace, workspace_bytes, status, false,
                     static_cast<cudaStream_t>(stream));
 }
 
@@ -1115,8 +1131,8 @@ int mstar_sampler_lmhead_step_w4(const mstar_sampler_params_t *p, const void *hi
   int64_t smem = 0;
   int rc = mstar_sampler_plan(p, &cs, &smem);
   if (rc) return rc;
-  rc = mstar_lmhead_logits_w4(hidden, ld_hidden, p->B, w, const_cast<void *>(p->logits), p->dtype, p->ld, workspace,
-                              workspace_bytes, status, stream);
+  rc = w4::logits(hidden, ld_hidden, p->B, w, const_cast<void *>(p->logits), p->dtype, p->ld, workspace,
+                  workspace_bytes, status, (p->flags & MSTAR_FLAG_TEST_WITHHOLD) != 0, static_cast<cudaStream_t>(stream));
   return rc ? rc : mstar_sampler_step(p, stream);
 }
 

@@ -537,7 +537,9 @@ def lmhead_logits_w4(hidden: torch.Tensor, codes: torch.Tensor, scales: torch.Te
     [V, d / group] float32 or bfloat16, zeros uint8 of the same shape or None
     for 8.  fp32 sums, stored as float32 or bfloat16.  workspace: None takes
     fresh scratch from torch's allocator (safe on any stream and inside graph
-    capture), or pass lmhead_w4_workspace's."""
+    capture), or pass lmhead_w4_workspace's.  A bounded wait inside the kernel
+    that runs out leaves wrong logits and sets bit 1 of `status`, and says so
+    nowhere else: a caller that must know gives one and reads it."""
     w = _w4(codes, scales, zeros)
     dev = codes.device
     B = _check_hidden_w4(hidden, w, dev)
@@ -557,7 +559,8 @@ def lmhead_step_w4(hidden: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
                    zeros=None, status=None, workspace: torch.Tensor | None = None, **kw) -> N.Params:
     """lmhead_logits_w4 into `logits` [B, V] (written) and one sampling step
     on it (mstar_sampler_lmhead_step_w4).  The sampling keywords are
-    sampler_step's; the logits are read back from L2."""
+    sampler_step's; the logits are read back from L2.  status: the head's, as
+    for lmhead_logits_w4 (out_status is the sampling step's)."""
     w = _w4(codes, scales, zeros)
     dev = codes.device
     B = _check_hidden_w4(hidden, w, dev)

@@ -847,3 +847,31 @@ def test_w4_odd_numbers_of_blocks(V, d, g):
         for _ in range(3):
             assert torch.equal(first, k.lmhead_logits_w4(hidden[:B], codes, scales, zeros=zeros, status=status))
         assert status.item() == 0
+
+
+@pytest.mark.parametrize("g", [32, 64, 128])
+@pytest.mark.parametrize("B,V,d", [(1, 70000, 384), (16, 4099, 1024), (32, 20011, 640), (64, 20011, 1024), (128, 9001, 896),
+                                   (200, 9001, 512)])
+def test_w4_withheld_copy_runs_out(B, V, d, g):
+    """Each CTA's last copy of hidden rows is never issued (no bad address, no
+    copy in flight): the waits on it give up after their limit, the call
+    returns and sets the status bit, and the next call with the same scratch
+    is right."""
+    from mstar_rs_b200 import _native as N
+    from mstar_rs_b200 import kernel as k
+
+    codes, scales, zeros = w4_inputs(V, d, g, BF16, True, V)
+    hidden = torch.randn(B, d, device="cuda", generator=gen(d)).to(BF16)
+    logits = torch.zeros(B, V, device="cuda")
+    ids = torch.zeros(B, dtype=torch.int64, device="cuda")
+    ws = k.lmhead_w4_workspace(B, V, d, "cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kw = dict(zeros=zeros, status=status, workspace=ws, out_ids=ids, uniforms=torch.full((B,), 0.5, device="cuda"))
+    k.lmhead_step_w4(hidden, codes, scales, logits, flags=N.FLAG_TEST_WITHHOLD, **kw)
+    torch.cuda.synchronize()
+    assert status.item() == 1
+    status.zero_()
+    k.lmhead_step_w4(hidden, codes, scales, logits, **kw)
+    assert status.item() == 0
+    ref, tol = R.head(hidden, codes, scales, zeros, F32, parts=16)
+    near(logits, ref, tol)
