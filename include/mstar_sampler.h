@@ -327,8 +327,9 @@ int mstar_token_logprobs(const void *logits, int32_t dtype, int32_t N, int32_t V
  * lse[n])), of the logits' type; dlogits may be logits itself (replaced in
  * place), otherwise it must not overlap it.  lse is mstar_token_logprobs', or
  * that of a longer row of which logits holds a part.  32 bits hold an lse to
- * 2^-24 of itself: from |lse| = 65536 on (every id of a row under a finite
- * mask), one that agrees with the row's own to that is replaced by it.
+ * 2^-24 of itself, which every probability of the row takes over: from |lse| =
+ * 256 on (f32; 32768 in bf16: every id of a row under a finite mask, or a small
+ * temperature), one that agrees with the row's own to that is replaced by it.
  * Padding and empty rows (lse -inf): zeros. */
 int mstar_token_logprobs_grad(const void *logits, int32_t dtype, int32_t N, int32_t V, int64_t ld, const int64_t *ids,
                               double temperature, const float *lse, const float *dlogp, void *dlogits,

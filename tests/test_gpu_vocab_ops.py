@@ -875,3 +875,36 @@ def test_w4_withheld_copy_runs_out(B, V, d, g):
     assert status.item() == 0
     ref, tol = R.head(hidden, codes, scales, zeros, F32, parts=16)
     near(logits, ref, tol)
+
+
+@pytest.mark.parametrize("n,V", [(4, 3001), (2, 70000)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradient_keeps_the_probabilities_of_large_lse(dtype, n, V):
+    """The gradient's probabilities at every size of lse: its rounding to 32
+    bits (2^-24 of itself) costs f32 gradients at most 2^-16 and bf16 ones, whose
+    own half step is 2^-8, 2^-9; larger ones are summed anew."""
+    from mstar_rs_b200 import kernel as k
+
+    limit = 256 if dtype == F32 else 2 ** 15
+    for T, shift in ((1.0, 150.0), (1.0, -1e4), (0.01, 0.0), (1.0, 300.0), (1.0, 20000.0), (0.5, -30000.0), (1.0, 65000.0)):
+        x = (torch.randn(n, V, device="cuda", generator=gen(n)) + shift).to(dtype)
+        x[1, 1::3] = -math.inf
+        ids = torch.randint(0, V // 3, (n,), device="cuda", generator=gen(1)) * 3
+        dlogp = torch.randn(n, device="cuda", generator=gen(2))
+        _, lse = k.token_logprobs(x, ids, temperature=T)
+        got = k.token_logprobs_grad(x, ids, lse, dlogp, temperature=T)
+        xd = x.double() / T
+        m = xd.amax(1, keepdim=True)
+        p = (xd - m).exp()
+        s = p.sum(1, keepdim=True)
+        p, true = p / s, (m + s.log())[:, 0]
+        hot = torch.zeros_like(p)
+        hot[torch.arange(n, device="cuda"), ids] = 1.0
+        g = (dlogp.double() / T)[:, None]
+        ref = g * (hot - p)
+        arg = torch.where(p > 0, (m - xd).clamp(max=1000) * 1.4427 * 2.0 ** -22, 0.0)
+        half = torch.where(true.abs() < limit, true.abs() * 2.0 ** -24, 0.0)[:, None]
+        tol = g.abs() * (p * (R.SUM + arg + half) + (hot + p) * 2.0 ** -23) + ref.abs() * R.HALF[dtype] + 2.0 ** -125 * (1 + g.abs())
+        near(got, ref, tol)
+        same = x.clone()
+        assert k.token_logprobs_grad(same, ids, lse, dlogp, temperature=T, out=same) is same and torch.equal(same, got)
