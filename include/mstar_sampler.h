@@ -271,9 +271,10 @@ typedef struct mstar_w4 {
  * minus zero point times hidden is exact; each group's sum is scaled in
  * fp32), stored as dtype.  Each hidden row enters as fp16 times a power of two:
  * exact for values down to 2^-32 of its largest, below that off by at most
- * 2^-40 of it.  NaN and infinities go where the products take them.  B <= 256.  workspace: device scratch of at least
- * mstar_lmhead_w4_workspace_bytes(B, V, d) bytes (which grow with B: the largest
- * batch's serves the smaller ones), 256-byte aligned; its
+ * 2^-40 of it.  NaN and infinities go where the products take them.  B <= 256.
+ * logits overlap neither the hidden rows nor the weights.  workspace: device
+ * scratch of at least mstar_lmhead_w4_workspace_bytes(B, V, d) bytes (which grow
+ * with B: the largest batch's serves the smaller ones), 256-byte aligned; its
  * contents need not be preserved or initialised, and calls that overlap on
  * the GPU need their own.  status: NULL or a device word that gets bit 1 if a
  * bounded in-kernel wait (0.1 s) ran out: some logits are then wrong or not
@@ -291,8 +292,8 @@ int mstar_sampler_lmhead_step_w4(const mstar_sampler_params_t *p, const void *hi
 
 /* Embedding lookup, the step's other end (the sampled ids' rows are the
  * next step's input): out[n, :] = scale * table[ids[n], :], out [N, d] of
- * out_dtype, table [V, ld] of dtype, or a 4-bit matrix (out 16-byte
- * aligned).  A negative id is a padding row and gives zeros; an id >= V
+ * out_dtype and apart from the table, table [V, ld] of dtype, or a 4-bit matrix
+ * (out 16-byte aligned).  A negative id is a padding row and gives zeros; an id >= V
  * does too and sets MSTAR_STATUS_BAD_ID in *status (NULL or a device word). */
 int mstar_embed_tokens(const int64_t *ids, int64_t N, const void *table, int32_t dtype, int32_t V, int32_t d,
                        int64_t ld, float scale, void *out, int32_t out_dtype, uint32_t *status, void *stream);

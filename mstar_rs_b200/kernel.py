@@ -501,6 +501,22 @@ def _w4(codes, scales, zeros) -> N.W4:
     return N.W4(codes.data_ptr(), scales.data_ptr(), zp, V, d, d // G, _DT[scales.dtype])
 
 
+def _apart(t, name, *read):
+    """Refuses an output that meets memory which the call reads: (tensor or None, what) each."""
+    a0 = t.data_ptr()
+    a1 = a0 + _extent(t)
+    for r, what in read:
+        if r is not None:
+            p = r.data_ptr()
+            if a0 < p + _extent(r) and p < a1:
+                raise ValueError(f"{name} must not overlap {what}")
+
+
+def _extent(t) -> int:
+    """_span, at the price of a multiplication for contiguous tensors."""
+    return t.nbytes if t.is_contiguous() else _span(t)
+
+
 def _check_hidden_w4(hidden, w, dev):
     if hidden.dtype != torch.bfloat16:
         raise TypeError(f"hidden must be bfloat16, got {hidden.dtype}")
@@ -547,6 +563,7 @@ def lmhead_logits_w4(hidden: torch.Tensor, codes: torch.Tensor, scales: torch.Te
         out = torch.empty(B, w.V, dtype=dtype, device=dev)
     else:
         _matrix(out, "out", dev, B, w.V)
+        _apart(out, "out", (hidden, "hidden"), (codes, "the codes"), (scales, "the scales"), (zeros, "the zeros"))
     if workspace is None:
         workspace = torch.empty(_w4_workspace_bytes(B, w.V, w.d, dev.index), dtype=torch.uint8, device=dev)
     wp, wn = _check_ws(workspace, dev)
@@ -565,6 +582,7 @@ def lmhead_step_w4(hidden: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     dev = codes.device
     B = _check_hidden_w4(hidden, w, dev)
     _matrix(logits, "logits", dev, B, w.V)
+    _apart(logits, "logits", (hidden, "hidden"), (codes, "the codes"), (scales, "the scales"), (zeros, "the zeros"))
     p = build_params(logits, **kw)
     if workspace is None:
         workspace = lmhead_w4_workspace(B, w.V, w.d, dev)
@@ -584,7 +602,7 @@ def _ids_1d(ids, dev):
     return ids.numel()
 
 
-def _lookup_out(ids, d, out, dtype, dev, table):
+def _lookup_out(ids, d, out, dtype, dev, *read):
     if out is None:
         if dtype not in _DT:
             raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
@@ -593,9 +611,7 @@ def _lookup_out(ids, d, out, dtype, dev, table):
         raise TypeError(f"out must be float32 or bfloat16, got {out.dtype}")
     if out.device != dev or out.shape != (*ids.shape, d) or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {(*ids.shape, d)} tensor on {dev}")
-    a0, b0 = out.data_ptr(), table.data_ptr()
-    if a0 < b0 + _span(table) and b0 < a0 + _span(out):
-        raise ValueError("out must not overlap the table")
+    _apart(out, "out", *read)
     return out
 
 
@@ -612,7 +628,7 @@ def embed_tokens(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, 
     V, d = table.shape
     _matrix(table, "table", dev, V, d)
     n = _ids_1d(ids, dev)
-    out = _lookup_out(ids, d, out, dtype or table.dtype, dev, table)
+    out = _lookup_out(ids, d, out, dtype or table.dtype, dev, (table, "the table"))
     st = _status(status, dev)
     if n:
         _call(dev, "mstar_embed_tokens", ids.data_ptr(), n, table.data_ptr(), _DT[table.dtype], V, d, _ld(table),
@@ -628,7 +644,7 @@ def embed_tokens_w4(ids: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
     w = _w4(codes, scales, zeros)
     dev = codes.device
     n = _ids_1d(ids, dev)
-    out = _lookup_out(ids, w.d, out, dtype, dev, codes)
+    out = _lookup_out(ids, w.d, out, dtype, dev, (codes, "the codes"), (scales, "the scales"), (zeros, "the zeros"))
     st = _status(status, dev)
     if n:
         _call(dev, "mstar_embed_tokens_w4", ids.data_ptr(), n, ctypes.byref(w), scale, out.data_ptr(), _DT[out.dtype],

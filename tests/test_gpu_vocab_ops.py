@@ -908,3 +908,47 @@ def test_gradient_keeps_the_probabilities_of_large_lse(dtype, n, V):
         near(got, ref, tol)
         same = x.clone()
         assert k.token_logprobs_grad(same, ids, lse, dlogp, temperature=T, out=same) is same and torch.equal(same, got)
+
+
+def test_w4_outputs_apart_from_their_inputs():
+    """An output that lies on what the call reads is refused before anything is
+    launched; one right beside it is not."""
+    from mstar_rs_b200 import kernel as k
+
+    V, d, B = 64, 128, 4
+    # one buffer: logits between the hidden rows and codes, scales and zeros
+    buf = torch.zeros(1 << 16, device="cuda", dtype=torch.uint8)
+    at, place = 0, {}
+    for name, n in (("hidden", B * d * 2), ("out", B * V * 4), ("codes", V * d // 2), ("scales", V * 4 * 4), ("zeros", V * 4)):
+        place[name] = at
+        at += n
+
+    def view(name, dtype, *shape, move=0):
+        n = math.prod(shape) * torch.tensor([], dtype=dtype).element_size()
+        return buf[place[name] + move:place[name] + move + n].view(dtype).view(*shape)
+
+    hidden, codes = view("hidden", BF16, B, d), view("codes", torch.uint8, V, d // 2)
+    scales, zeros = view("scales", F32, V, 4), view("zeros", torch.uint8, V, 4)
+    hidden.copy_(torch.randn(B, d, device="cuda", generator=gen(1)))
+    for t, u in zip((codes, scales, zeros), w4_inputs(V, d, 32, F32, True, 2)):
+        t.copy_(u)
+    keep = buf.clone()
+    ids = torch.tensor([3, -1], device="cuda")
+    step = dict(zeros=zeros, out_ids=torch.zeros(B, dtype=torch.int64, device="cuda"),
+                uniforms=torch.full((B,), 0.5, device="cuda"))
+    for name, move, what in (("out", -4, "hidden"), ("out", 16, "codes"), ("codes", 0, "codes"), ("scales", -16, "codes"),
+                             ("scales", 16, "scales"), ("zeros", 64, "zeros")):
+        with pytest.raises(ValueError, match=what):
+            k.lmhead_logits_w4(hidden, codes, scales, zeros=zeros, out=view(name, F32, B, V, move=move))
+        with pytest.raises(ValueError, match=what):
+            k.lmhead_step_w4(hidden, codes, scales, view(name, F32, B, V, move=move), **step)
+    for name, move, what in (("codes", 64, "codes"), ("scales", 32, "scales"), ("zeros", 64, "zeros")):
+        with pytest.raises(ValueError, match=what):
+            k.embed_tokens_w4(ids, codes, scales, zeros=zeros, out=view(name, F32, 2, d, move=move))
+    assert torch.equal(buf, keep)
+    out = view("out", F32, B, V)
+    k.lmhead_logits_w4(hidden, codes, scales, zeros=zeros, out=out)
+    assert torch.equal(out, k.lmhead_logits_w4(hidden.clone(), codes.clone(), scales.clone(), zeros=zeros.clone()))
+    row = view("out", F32, 2, d)
+    k.embed_tokens_w4(ids, codes, scales, zeros=zeros, out=row)
+    assert torch.equal(row, k.embed_tokens_w4(ids, codes.clone(), scales.clone(), zeros=zeros.clone(), dtype=F32))
