@@ -560,6 +560,8 @@ def lmhead_logits_w4(hidden: torch.Tensor, codes: torch.Tensor, scales: torch.Te
     dev = codes.device
     B = _check_hidden_w4(hidden, w, dev)
     if out is None:
+        if dtype not in _DT:
+            raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
         out = torch.empty(B, w.V, dtype=dtype, device=dev)
     else:
         _matrix(out, "out", dev, B, w.V)

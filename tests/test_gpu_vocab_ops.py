@@ -952,3 +952,18 @@ def test_w4_outputs_apart_from_their_inputs():
     row = view("out", F32, 2, d)
     k.embed_tokens_w4(ids, codes, scales, zeros=zeros, out=row)
     assert torch.equal(row, k.embed_tokens_w4(ids, codes.clone(), scales.clone(), zeros=zeros.clone(), dtype=F32))
+
+
+def test_w4_outputs_of_another_type():
+    """A type that the logits or rows cannot have is a TypeError, as in every
+    other call."""
+    from mstar_rs_b200 import kernel as k
+
+    codes, scales, zeros = w4_inputs(64, 128, 32, F32, True, 1)
+    for dt in (torch.float16, torch.float64, torch.int32):
+        with pytest.raises(TypeError):
+            k.lmhead_logits_w4(torch.zeros(4, 128, device="cuda", dtype=BF16), codes, scales, dtype=dt)
+        with pytest.raises(TypeError):
+            k.embed_tokens_w4(torch.zeros(4, dtype=torch.int64, device="cuda"), codes, scales, dtype=dt)
+        with pytest.raises(TypeError):
+            k.embed_tokens_grad(torch.zeros(4, dtype=torch.int64, device="cuda"), torch.zeros(4, 8, device="cuda"), 9, dtype=dt)
