@@ -468,7 +468,7 @@ def quantize_w4(weight: torch.Tensor, group_size: int = 128, *, zero_points: boo
     if scale_dtype not in _DT:
         raise TypeError("scale_dtype must be float32 or bfloat16")
     V, d = weight.shape
-    w = weight.detach().float().view(V, d // group_size, group_size)
+    w = weight.detach().float().contiguous().view(V, d // group_size, group_size)
     if zero_points:
         lo, hi = w.amin(2).clamp(max=0), w.amax(2).clamp(min=0)
         scales = ((hi - lo) / 15).to(scale_dtype)

@@ -226,3 +226,15 @@ def test_embed_grad_workspace_of_more_tokens_serves_fewer(d):
     counts = list(range(1, 4000)) + list(range(4000, 400000, 37))
     sizes = [lib.mstar_embed_grad_workspace_bytes(n, 4099, d) for n in counts]
     assert sizes[0] > 0 and all(a <= b for a, b in zip(sizes, sizes[1:]))
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+def test_quantize_w4_of_views(zero_points):
+    """A transposed weight, and one inside a wider matrix, give what their
+    copies give, in the contiguous rows that the calls ask for."""
+    wide = torch.randn(256, 300, generator=torch.Generator().manual_seed(5))
+    for w in (wide.t()[:, :128], wide[3:50, 7:135], wide.bfloat16().t()[::2, 64:192]):
+        got = kernel.quantize_w4(w, 32, zero_points=zero_points)
+        want = kernel.quantize_w4(w.contiguous(), 32, zero_points=zero_points)
+        for a, b in zip(got, want):
+            assert (a is None and b is None) or (a.is_contiguous() and torch.equal(a, b))
