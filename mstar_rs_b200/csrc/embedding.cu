@@ -38,23 +38,31 @@ namespace emb {
 
 constexpr int NT = 256;
 
+// A load of memory that the kernel only reads (RO), or of any.
+template <bool RO, typename A>
+__device__ __forceinline__ A get(const A *p) {
+  if constexpr (RO)
+    return __ldg(p);
+  else
+    return *p;
+}
 // W consecutive values as one access (W = 8: 16 bytes of bf16, two of 16 of f32).
-template <int W>
+template <int W, bool RO = true>
 __device__ __forceinline__ void load(const float *p, float (&x)[W]) {
   if constexpr (W == 8) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    const float4 a = get<RO>(reinterpret_cast<const float4 *>(p)), b = get<RO>(reinterpret_cast<const float4 *>(p) + 1);
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
   } else if constexpr (W == 2) {
-    const float2 a = __ldg(reinterpret_cast<const float2 *>(p));
+    const float2 a = get<RO>(reinterpret_cast<const float2 *>(p));
     x[0] = a.x, x[1] = a.y;
   } else {
-    x[0] = __ldg(p);
+    x[0] = get<RO>(p);
   }
 }
-template <int W>
+template <int W, bool RO = true>
 __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&x)[W]) {
   if constexpr (W == 8) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint4 a = get<RO>(reinterpret_cast<const uint4 *>(p));
     const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -62,7 +70,7 @@ __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&x)[W]) {
       x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
     }
   } else if constexpr (W == 2) {
-    const uint32_t u = __ldg(reinterpret_cast<const uint32_t *>(p));
+    const uint32_t u = get<RO>(reinterpret_cast<const uint32_t *>(p));
     x[0] = __uint_as_float(u << 16);
     x[1] = __uint_as_float(u & 0xFFFF0000u);
   } else {
@@ -394,9 +402,10 @@ __global__ void __maxnreg__(40) sort_tokens_kernel(const Grad a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// (base may be the output, whose rows this kernel writes: no read-only load)
 template <typename TO, int W>
 __device__ __forceinline__ void load_base(const Grad &a, int v, int col, float (&b)[W]) {
-  if (a.base) load<W>(static_cast<const TO *>(a.base) + (int64_t)v * a.d + col, b);
+  if (a.base) load<W, false>(static_cast<const TO *>(a.base) + (int64_t)v * a.d + col, b);
 }
 template <typename TO, int W>
 __device__ __forceinline__ void finish(const Grad &a, int v, int col, float (&acc)[W], const float (&b)[W]) {
