@@ -967,3 +967,74 @@ def test_w4_outputs_of_another_type():
             k.embed_tokens_w4(torch.zeros(4, dtype=torch.int64, device="cuda"), codes, scales, dtype=dt)
         with pytest.raises(TypeError):
             k.embed_tokens_grad(torch.zeros(4, dtype=torch.int64, device="cuda"), torch.zeros(4, 8, device="cuda"), 9, dtype=dt)
+
+
+@pytest.mark.parametrize("V,d", [(1, 1), (40, 3), (37, 64), (500, 501), (3000, 128)])
+@pytest.mark.parametrize("ot", [BF16, F32])
+def test_embed_grad_at_any_address(V, d, ot):
+    """Outputs and bases that start off a 16-byte border, at the same place
+    modulo 16 bytes and at different ones: the definition's values, and nothing
+    before or behind the output is written."""
+    from mstar_rs_b200 import kernel as k
+
+    n = 2 * V + 5
+    ids = torch.randint(-1, V + 1, (n,), device="cuda", generator=gen(V))
+    dout = torch.randn(n, d, device="cuda", generator=gen(d)).to(BF16)
+    base = torch.randn(V, d, device="cuda", generator=gen(3)).to(ot)
+    fresh = {False: k.embed_tokens_grad(ids, dout, V, dtype=ot), True: k.embed_tokens_grad(ids, dout, V, base=base, dtype=ot)}
+    for kind, got in fresh.items():
+        ref, tol = R.embed_grad(ids, dout, V, 1.0, base if kind else None, ot)
+        near(got, ref, tol)
+
+    def at(places):
+        buf = torch.full((V * d + 32,), 5.0, device="cuda").to(ot)
+        return buf, buf[places:places + V * d].view(V, d)
+
+    for i in range(0, 9):
+        buf, out = at(i)
+        k.embed_tokens_grad(ids, dout, V, out=out)
+        assert torch.equal(out, fresh[False])
+        assert bool((buf[:i] == 5).all()) and bool((buf[i + V * d:] == 5).all())
+        for j in (i, i + 1, 8 - i):
+            buf, out = at(i)
+            keep, b = at(j)
+            b.copy_(base)
+            k.embed_tokens_grad(ids, dout, V, base=b, out=out)
+            assert torch.equal(out, fresh[True]) and torch.equal(b, base)
+            assert bool((buf[:i] == 5).all()) and bool((buf[i + V * d:] == 5).all())
+        buf, out = at(i)
+        out.copy_(base)
+        k.embed_tokens_grad(ids, dout, V, base=out, out=out)
+        assert torch.equal(out, fresh[True])
+        assert bool((buf[:i] == 5).all()) and bool((buf[i + V * d:] == 5).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_lmhead_step_w4_against_the_oracle(oracle_lib, dtype):
+    """The one call at full size: its logits against the 4-bit definition, and
+    the ids that the oracle takes from those logits."""
+    import numpy as np
+
+    from mstar_rs_b200 import kernel as k
+    from mstar_rs_b200 import workloads as W
+
+    B, V, d = 64, 151936, 2048
+    case = W.qwen_mixed(seed=8, B=B, V=V)
+    case.dtype = dtype
+    kw = W.to_device(case)
+    kw.pop("logits")
+    codes, scales, z = w4_inputs(V, d, 128, BF16, True, 6)
+    scales *= 4  # (logits of some units, so that the cuts of top_p and min_p are met)
+    hidden = torch.randn(B, d, device="cuda", generator=gen(4)).to(BF16)
+    tdt = BF16 if dtype == "bf16" else F32
+    logits = torch.empty(B, V, dtype=tdt, device="cuda")
+    ids = torch.zeros(B, dtype=torch.int64, device="cuda")
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    k.lmhead_step_w4(hidden, codes, scales, logits, zeros=z, status=st, **kw, out_ids=ids)
+    assert st.item() == 0
+    for v in range(0, V, 30000):  # (in parts: the definition is in 64 bits)
+        part = slice(v, min(V, v + 30000))
+        ref, tol = R.head(hidden, codes[part], scales[part], z[part], tdt, parts=16)
+        near(logits[:, part], ref, tol)
+    case.logits = logits.float().cpu().numpy() if dtype == "f32" else logits.view(torch.int16).cpu().numpy().view(np.uint16)
+    assert np.array_equal(ids.cpu().numpy(), oracle_lib.run(case)["ids"])
