@@ -88,6 +88,9 @@ struct Roles {
   static constexpr int COUNTER = REST > 2 + ISSUE ? 2 + ISSUE : 1;
   static constexpr int THREADS = 32 * (EXPAND + SUM + REST);
   static constexpr int LAUNCH = 65536 / THREADS / 8 * 8;
+  // What they hold fits but for four of the twelve variants: at 128 columns expanders
+  // (56) and accumulators (160: 128 sums, 16 values read) spill 216, 152 and 32 bytes
+  // with groups of 32, 64 and 128, at 64 columns with groups of 32 both spill 60.
   static constexpr int REGS_EXPAND = N > 64 ? 56 : 64;
   static constexpr int REGS_SUM = N > 64 ? 160 : 80;
   static constexpr int REGS_REST = 48;
@@ -645,7 +648,10 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
   constexpr int RING = R::RING;
   constexpr bool MERGED = R::template merged<GPB>();
   constexpr int NC = N / R::HALVES;       // this warp's columns, from `from`
-  constexpr int LC = N == 32 || N == 64 ? 32 : 16;  // columns loaded at a time
+  // Columns loaded at a time.  With groups below 128, 32 of them would not fit the
+  // registers beside the scales (32 rows, V=151936, d=2048: groups of 32 127 us with
+  // 32 columns and spills, 118 with 16; groups of 64 85 and 77).
+  constexpr int LC = GPB == 1 && (N == 32 || N == 64) ? 32 : 16;
   const int warp = (int)(threadIdx.x >> 5) - R::EXPAND, lane = threadIdx.x & 31;
   const int t = (warp >> 2) & 1, quad = warp & 3, row = t * 128 + quad * 32 + lane, from = (warp >> 3) * NC;
   const uint32_t at0 = tbase + ((uint32_t)(quad * 32) << 16) + R::D_COL + (uint32_t)(t * N + from);
