@@ -33,14 +33,16 @@
 // instructions and an arrival cost each role some hundred cycles, next to the
 // 735 in which memory delivers a block of 256 x 128 codes.  So the two blocks
 // of a stage have an A buffer, accumulators, expander warps and issuers of
-// their own (up to 32 batch rows), each of which has twice the time; with
-// groups of 128 one barrier says that A is written and the accumulator free,
-// and one that both are done with.
+// their own (up to 32 batch rows), each of which has twice the time.  Above 64
+// rows, where each half of the tile has one accumulator, groups of 128 take one
+// barrier for A written and the accumulator free and one for both done with.
 //
 // A word holds eight codes; codes i and i + 4 are a pair: one instruction masks
 // them and sets fp16's exponent (0x6400 | q is 1024 + q; at bits 4-7 it is
 // 1024 + 16 q), one subtracts.  The pairs' order is [0 4 1 5 2 6 3 7] and the
-// kernel before puts the hidden columns into it.
+// kernel before puts the hidden columns into it.  (Codes beside fp16's exponent of
+// 1024 are a known way from 4 bits to fp16: Kim et al., "Who Says Elephants Can't
+// Run: Bringing Large Scale MoE Models into Cloud Scale Production", 2022.)
 //
 // A tile that several CTAs share is summed by the one whose part comes last, in
 // the order of the columns: no CTA waits for another, and the sum does not
@@ -102,11 +104,13 @@ struct Roles {
   static constexpr int D_COL = 256;
   static constexpr int SLOTS = N > 64 ? 1 : N > 32 ? 2 : 4;
   static constexpr int RING = SLOTS / LANES;  // slots per lane
-  // One barrier for A written and the accumulator free, one for both done.
+  // One barrier for A written and the accumulator free, one for both done: where
+  // a block has one group and the one accumulator (128 columns alone).
   template <int GPB>
   static __host__ __device__ constexpr bool merged() {
     return GPB == 1 && RING == 1;
   }
+  static_assert(LANES == 1 || RING > 1, "merged barriers are written for one lane");
 };
 constexpr int MAX_WS = 6, MAX_HS = 8;
 constexpr int MAX_N = 128;         // batch rows per chunk
@@ -184,10 +188,10 @@ __device__ __forceinline__ void sharers(const Gemm &g, int tile, int &c_lo, int 
 
 struct Sh {
   uint64_t wfull[MAX_WS], wempty[MAX_WS], hfull[MAX_HS], hempty[MAX_HS];
-  // By half of the tile t and block of the stage j.  Groups of 128 (one per
-  // block): ready[t][j] = A written and the block's accumulator free,
-  // done[t][j] = its MMAs complete.  Smaller groups: ready is A's alone and
-  // done frees it, dfull and dempty [t][slot] hand the accumulators over.
+  // By half of the tile t and block of the stage j: ready[t][j] = A written,
+  // done[t][j] = its MMAs complete; dfull and dempty [t][slot] hand the
+  // accumulators over.  Merged (128 columns, groups of 128): ready also says that
+  // the accumulator is free, and done that its sums are there.
   uint64_t ready[2][2], done[2][2], dfull[2][4], dempty[2][4], mma_done[4];
   uint32_t tmem_base;
   int abort;
@@ -475,7 +479,7 @@ __device__ void issue(const Gemm &g, Sh &sh, uint8_t *sH, uint32_t tbase, int wh
         const uint32_t lo = hlo + at * 2u * box16, aj = a0 + (uint32_t)j * 128u;
         if (MERGED) {
           tc_fence_after();
-          mma_group<KB>(lead, d0 + (R::LANES == 2 ? j : 0) * 2u * N, aj, lo, hhi, box16, idesc);
+          mma_group<KB>(lead, d0, aj, lo, hhi, box16, idesc);
         } else {
           const int groups = GPB == 1 ? 1 : min(GPB, (g.d - (2 * k + j) * KB) / (KB / GPB));
 #pragma unroll
@@ -668,8 +672,7 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
   const uint32_t ready = smem_u32(sh.ready[t]), dempty = smem_u32(sh.dempty[t]);
   uint32_t fp = 0, late = 0;  // parities of done[t][j] (groups of 128) or dfull[t][slot], a bit each
   int slot = 0;
-  if (MERGED)  // the first blocks' accumulators are free
-    for (int j = 0; j < R::LANES; ++j) arrive(ready + 8u * j, lane0);
+  if (MERGED) arrive(ready, lane0);  // the first block's accumulator is free
   Work w(g);
   while (w.next(g)) {
     const int v = w.tile / g.nchunks * BM + row, chunk = w.tile % g.nchunks;
@@ -755,10 +758,8 @@ __device__ void sum_rows(const Gemm &g, Sh &sh, uint32_t tbase) {
             tmem_wait_ld();
             if (c0 + LC == NC) {  // all is in registers: the accumulator is free
               tc_fence_before();
-              // (with one lane it is the next block's, otherwise this lane's next)
-              arrive(!MERGED ? dempty + 8u * q
-                             : ready + 8u * (R::LANES == 2 ? j : j == 0 && b + 1 < g.nblk ? 1 : 0),
-                     lane0);
+              // (merged: for the next block)
+              arrive(!MERGED ? dempty + 8u * q : ready + 8u * (j == 0 && b + 1 < g.nblk ? 1 : 0), lane0);
             }
             float scale;
             if constexpr (!WORDS) {
