@@ -972,11 +972,21 @@ static Gemm plan(int B, int V, int d) {
 // them adds: a divisor of the stages at or above their square root (16 x 1024 x
 // 4096: 20.5 us with sixteen parts, 15.3 with four).  Up to seven stages one unit
 // per CTA is quicker (16 x 4099 x 1024: 12.3 us with four parts, 13.4 with two).
+// Where the least such divisor is more than twice the root (a prime number of
+// stages has itself alone), six parts, or the root where that is more, although
+// shares then differ by a unit: 11, 13, 17, 19 and 23 stages, 16 rows, V=2048 16.4,
+// 18.6, 24.0, 24.3 and 28.3 us with a part per stage, 16.4, 16.5, 18.1, 18.8 and
+// 20.3 with six.  (A divisor that is near is quicker: 15 stages 16.1 us with five
+// parts, 19.0 with four.)
 static int grid_of(const Gemm &g) {
   int parts = g.nks;
-  if (g.nks >= 8)
-    for (int p = g.nks - 1; p * p >= g.nks; --p)
+  if (g.nks >= 8) {
+    int root = 1;
+    while (root * root < g.nks) ++root;
+    for (int p = g.nks - 1; p >= root; --p)
       if (g.nks % p == 0) parts = p;
+    if (parts * parts > 4 * g.nks) parts = std::max(6, root);
+  }
   return (int)std::min<int64_t>(sm_count(), (int64_t)g.ntt * parts);
 }
 

@@ -1038,3 +1038,18 @@ def test_lmhead_step_w4_against_the_oracle(oracle_lib, dtype):
         near(logits[:, part], ref, tol)
     case.logits = logits.float().cpu().numpy() if dtype == "f32" else logits.view(torch.int16).cpu().numpy().view(np.uint16)
     assert np.array_equal(ids.cpu().numpy(), oracle_lib.run(case)["ids"])
+
+
+@pytest.mark.parametrize("stages,V", [(11, 700), (13, 2000), (17, 300), (19, 4099), (22, 1000), (23, 257), (37, 600)])
+def test_w4_stages_without_a_near_divisor(stages, V):
+    """Widths whose stages do not divide evenly over a tile's CTAs."""
+    from mstar_rs_b200 import kernel as k
+
+    for d in (stages * 256, stages * 256 - 128):
+        codes, scales, zeros = w4_inputs(V, d, 64, F32, True, d)
+        hidden = torch.randn(40, d, device="cuda", generator=gen(V)).to(BF16)
+        ref, tol = R.head(hidden, codes, scales, zeros, F32, parts=16)
+        for B in (1, 16, 40):
+            out = k.lmhead_logits_w4(hidden[:B], codes, scales, zeros=zeros)
+            near(out, ref[:B], tol[:B])
+            assert torch.equal(out, k.lmhead_logits_w4(hidden[:B], codes, scales, zeros=zeros))
