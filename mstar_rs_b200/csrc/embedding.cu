@@ -629,15 +629,18 @@ static int sort_bins(int V) { return (((V + (1 << sort_log2(V)) - 1) >> sort_log
 
 // Workspace: start [C * bins + 1], pos [N], key [N], part [nchunks][2][d], each
 // rounded to 256 bytes.
+// The chunks' length is an order of additions and a size of scratch, so it goes by
+// a B200's 148 SMs and not by those that the current device shows.
+constexpr int SMS = 148;
 struct Layout {
-  int chunk, nchunks, cols;
+  int chunk, nchunks;
   int64_t start, pos, key, part, bytes;
 };
 static Layout layout(int N, int V, int d) {
   Layout l{};
   // chunks long enough to amortise a border, short enough for some waves of CTAs
   const int64_t tiles = (d + SUM_NT * 8 - 1) / (SUM_NT * 8);
-  l.chunk = (int)std::min<int64_t>(MAX_CHUNK, std::max<int64_t>(32, (int64_t)N * tiles / (148 * 16)));
+  l.chunk = (int)std::min<int64_t>(MAX_CHUNK, std::max<int64_t>(32, (int64_t)N * tiles / (SMS * 16)));
   l.nchunks = (N + l.chunk - 1) / l.chunk;
   const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
   l.start = 0;
@@ -645,9 +648,11 @@ static Layout layout(int N, int V, int d) {
   l.key = l.pos + up((int64_t)N * 4);
   l.part = l.key + up((int64_t)N * 4);
   // parts: as many as any batch of up to N tokens has (the chunks' length grows
-  // with N between 32 and 128, where their number stays near 2368 / tiles), so
-  // that a workspace for the largest batch serves the smaller ones
-  const int64_t most = std::min<int64_t>((N + 31) / 32, std::max<int64_t>(2442 / tiles + 3, (N + 127) / 128));
+  // with N between 32 and 128, where their number stays near 16 SMS / tiles, at
+  // most a 32nd above it), so that a workspace for the largest batch serves the
+  // smaller ones
+  const int64_t most =
+      std::min<int64_t>((N + 31) / 32, std::max<int64_t>(SMS * 16 * 33 / 32 / tiles + 3, (N + 127) / 128));
   l.bytes = l.part + up(std::max<int64_t>(most, l.nchunks) * 2 * d * 4);
   return l;
 }
@@ -687,7 +692,7 @@ static int launch_grad(Grad &a, cudaStream_t st) {
     e = cudaLaunchKernelEx(&cfg, sum_tokens_kernel<TI, TO, W>, a);
   }
   if (e == cudaSuccess && a.nchunks > 1) {
-    cfg.gridDim = dim3((unsigned)std::min(a.nchunks - 1, 148), (unsigned)a.col_tiles, 1);
+    cfg.gridDim = dim3((unsigned)std::min(a.nchunks - 1, sm_count()), (unsigned)a.col_tiles, 1);
     cfg.blockDim = dim3(SUM_NT * JOIN_G, 1, 1);
     e = cudaLaunchKernelEx(&cfg, join_tokens_kernel<TO, W>, a);
   }
