@@ -44,13 +44,13 @@ constexpr int NT = 256;
 constexpr int NW = NT / 32;
 constexpr int MAX_S = 8;                  // portable cluster width
 constexpr int SLICE_BYTES = 80 * 1024;  // of a row per CTA, where there are rows enough
-// Values at or below FLOOR count as masked while the running maximum is
-// tracked (a mask of the type's lowest value would overflow when scaled by
-// c).  A row whose scaled maximum M is not inside (-EDGE, EDGE) takes the exact
-// path, which subtracts before it scales: terms carry M's rounding, at most 2^5
-// below EDGE = 2^30, but from 2^32 on it leaves the exponent's range (a row whose
-// every id is masked by -1e10).
-constexpr float FLOOR = -1e30f;
+// Terms carry the rounding of the scaled maximum M, at most 2^5 below EDGE = 2^30,
+// but from 2^32 on it leaves the exponent's range.  So a row whose M is not inside
+// (-EDGE, EDGE) takes the exact path, which subtracts before it scales (a row whose
+// every id is masked by -1e10), and a running maximum starts at -EDGE and not below
+// it: a thread may meet masked ids alone before the first other one, and a sum that
+// has left the range does not come back when the maximum rises.  Beside -EDGE,
+// which is exact, a masked id's term is 1 at most.
 constexpr float EDGE = 0x1p30f;
 
 enum : int { LOGPROBS = 0, POLICY = 1, POLICY_GRAD = 2 };
@@ -61,6 +61,7 @@ struct Args {
   int32_t N, V, S;
   const int64_t *ids;
   float c;             // log2(e) / T
+  float floor;         // -EDGE / c
   double inv_t;
   float *logp, *lse, *loss;
   void *dlogits;
@@ -167,7 +168,7 @@ __device__ __forceinline__ void each_vector(int first, int end, Load load, F f) 
 // Running (maximum, sum) in scaled units: s = sum 2^(x c - M), in two halves.
 struct Stat {
   float m, M, s0, s1;  // raw maximum, scaled maximum, sums
-  __device__ explicit Stat(float c) : m(FLOOR), M(FLOOR * c), s0(0.f), s1(0.f) {}
+  __device__ explicit Stat(float floor) : m(floor), M(-EDGE), s0(0.f), s1(0.f) {}
   __device__ __forceinline__ void raise(float mx, float c) {
     if (mx > m) {
       const float M2 = mx * c, f = ex2(M - M2);
@@ -426,7 +427,7 @@ __global__ void __launch_bounds__(NT, 6) token_rows_kernel(const Args a) {
   if (tid < 32) tok = Token::read<MODE>(a, row, x_id);
   const float x_fringe = fringe >= 0 ? to_f(in.p[fringe]) : 0.f;
   const float c = a.c;
-  Stat st(c);
+  Stat st(a.floor);
   // (a gradient reads the slice again, from L2: the rows in flight are some
   // tens of megabytes; otherwise it is read once)
   each_vector<U>(
@@ -680,6 +681,10 @@ static void set_temperature(double temperature, float &c, double &inv_t) {
   inv_t = 1.0 / temperature;
   c = (float)(1.4426950408889634074 * inv_t);
 }
+static void set_temperature(double temperature, Args &a) {
+  set_temperature(temperature, a.c, a.inv_t);
+  a.floor = -EDGE / a.c;
+}
 
 }  // namespace rows
 }  // namespace mstar
@@ -699,7 +704,7 @@ int mstar_token_logprobs(const void *logits, int32_t dtype, int32_t N, int32_t V
   a.N = N;
   a.V = V;
   a.ids = ids;
-  rows::set_temperature(temperature, a.c, a.inv_t);
+  rows::set_temperature(temperature, a);
   a.logp = logp;
   a.lse = lse;
   a.status = status;
@@ -760,7 +765,7 @@ int mstar_policy_loss(const mstar_policy_params_t *p, void *stream) {
   a.N = p->N;
   a.V = p->V;
   a.ids = p->ids;
-  rows::set_temperature(p->temperature, a.c, a.inv_t);
+  rows::set_temperature(p->temperature, a);
   a.logp = p->logp;
   a.lse = p->lse;
   a.loss = p->loss;

@@ -1053,3 +1053,49 @@ def test_w4_stages_without_a_near_divisor(stages, V):
             out = k.lmhead_logits_w4(hidden[:B], codes, scales, zeros=zeros)
             near(out, ref[:B], tol[:B])
             assert torch.equal(out, k.lmhead_logits_w4(hidden[:B], codes, scales, zeros=zeros))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [5000, 22357, 151936])
+def test_rows_under_finite_masks(V, dtype):
+    """Masks of every finite size over most of a row, in the front of it, the
+    back or throughout, at every temperature: the ids left have the whole
+    probability, masked ones none."""
+    from mstar_rs_b200 import kernel as k
+
+    n = 6
+    for mask in (-1e4, -1e9, -1e10, -1e15, -1e25, -1e30, -1e35, torch.finfo(dtype).min):
+        for T in (1.0, 0.3, 0.01, 1e-5, 1e5):
+            G = gen(V)
+            x = torch.randn(n, V, device="cuda", generator=G).to(dtype)
+            hide = torch.rand(n, V, device="cuda", generator=G) < 0.999
+            hide[1, :-9], hide[1, -9:] = True, False   # the front
+            hide[2, :9], hide[2, 9:] = False, True     # the back
+            hide[3] = True
+            hide[3, V // 2] = False                    # all but one
+            hide[4] = False
+            hide[:, V // 3] = False
+            x = torch.where(hide, mask, x.double()).to(dtype)
+            ids = torch.full((n,), V // 3, device="cuda")
+            logp, lse = k.token_logprobs(x, ids, temperature=T)
+            _, rl, rp = R.rows(x, ids, T)
+            near(lse, rl.clamp(-3.4028234e38, 3.4028234e38), R.SUM + rl.abs() * 2.0 ** -23)
+            near(logp, rp, R.SUM + rp.abs() * 2.0 ** -23)
+            one = torch.ones(n, device="cuda")
+            loss, lp2, dx = k.policy_loss(x, ids, None, -one, temperature=T)  # r = 1, A = -1: loss 1, gradient of logp
+            assert torch.equal(lp2, logp) and bool((loss == 1).all())
+            g = k.token_logprobs_grad(x, ids, lse, one, temperature=T)
+            xd = x.double() / T
+            m = xd.amax(1, keepdim=True)
+            p = (xd - m).exp()
+            p = p / p.sum(1, keepdim=True)
+            ref = -p / T
+            ref[:, V // 3] += 1 / T
+            arg = torch.where(p > 0, (m - xd).clamp(max=1000) * 1.4427 * 2.0 ** -22, 0.0)
+            limit = 256 if dtype == F32 else 2 ** 15
+            half = torch.where(rl.abs() < limit, rl.abs() * 2.0 ** -24, 0.0)[:, None]
+            # (the id's own place is off by what its probability and 1 are)
+            tol = (p * (R.SUM + arg) + p * 2.0 ** -22) / T + ref.abs() * R.HALF[dtype] + 2.0 ** -125 * (1 + 1 / T)
+            tol[:, V // 3] += 2.0 ** -23 / T
+            near(dx, ref, tol)
+            near(g, ref, tol + p * half / T)
