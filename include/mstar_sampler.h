@@ -271,7 +271,8 @@ typedef struct mstar_w4 {
  * minus zero point times hidden is exact; each group's sum is scaled in
  * fp32), stored as dtype.  Each hidden row enters as fp16 times a power of two:
  * exact for values down to 2^-32 of its largest, below that off by at most
- * 2^-40 of it.  NaN and infinities go where the products take them.  B <= 256.
+ * 2^-40 of it; the sums are kept in that scaling, so scales stay below 2^88.
+ * NaN and infinities go where the products take them.  B <= 256.
  * logits overlap neither the hidden rows nor the weights.  workspace: device
  * scratch of at least mstar_lmhead_w4_workspace_bytes(B, V, d) bytes (which grow
  * with B: the largest batch's serves the smaller ones), 256-byte aligned; its
